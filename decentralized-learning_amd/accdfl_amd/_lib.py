@@ -19,6 +19,9 @@ import numpy as np
 PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))  # decentralized-learning_amd/
 REPO_ROOT = os.path.dirname(PKG_ROOT)
 CSRC = os.path.join(PKG_ROOT, "csrc", "dlagg.hip")
+# norms and norm bounds: a translation unit of its own, linked into the same library
+CSRC_BOUND = os.path.join(PKG_ROOT, "csrc", "bound.hip")
+CSRC_INTERNAL = os.path.join(PKG_ROOT, "csrc", "dlagg_internal.h")
 INCLUDE = os.path.join(REPO_ROOT, "include")
 HEADER = os.path.join(INCLUDE, "dlagg.h")
 # ACCDFL_AMD_TUNING=1 loads the tuning build (lib/libdlagg_tuning.so, -DDLA_TUNING=1: the same library
@@ -49,6 +52,9 @@ HIPCC_FLAGS = [
     "-fPIC",
     "-shared",
 ]
+# bound.hip: no packed FP32 instructions (some of their forms have given wrong results on this chip; its
+# arithmetic is in 64 bits and loses nothing)
+BOUND_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 EXPORTED = (
     "dla_version",
@@ -84,6 +90,13 @@ EXPORTED = (
     "dla_host_in_place_rounds",
     "dla_wsum_multi_table_acc",
     "dla_wsum_mixed",
+    "dla_norm_workspace",
+    "dla_norm",
+    "dla_norm_scale",
+    "dla_peer_workspace",
+    "dla_peer_norms",
+    "dla_wsum_bounded",
+    "dla_wsum_bounded_slab_tiled",
 )
 
 
@@ -92,14 +105,14 @@ class DlaggError(RuntimeError):
 
 
 def source_build_id(tuning: bool = False) -> str:
-    """Hash of the sources and flags libdlagg.so is built from (csrc/dlagg.hip,
+    """Hash of the sources and flags libdlagg.so is built from (csrc/dlagg.hip, csrc/bound.hip,
     include/dlagg.h, HIPCC_FLAGS; the tuning build's flag too).  build() compiles it into the
     library, and lib() refuses a library whose dla_build_id() differs from the tree's."""
     h = hashlib.sha256()
-    for path in (CSRC, HEADER):
+    for path in (CSRC, CSRC_BOUND, CSRC_INTERNAL, HEADER):
         with open(path, "rb") as f:
             h.update(f.read())
-    h.update(" ".join(HIPCC_FLAGS + (_TUNING_FLAGS if tuning else [])).encode())
+    h.update(" ".join(HIPCC_FLAGS + BOUND_FLAGS + (_TUNING_FLAGS if tuning else [])).encode())
     return h.hexdigest()[:20]
 
 
@@ -124,8 +137,9 @@ def file_build_id(path: str, prefix: bytes = _ID_PREFIX) -> Optional[str]:
 
 
 def build(force: bool = False, verbose: bool = False, tuning: bool = False) -> str:
-    """Compile csrc/dlagg.hip for gfx950 into lib/libdlagg.so (in-tree; tuning=True: the A/B build,
-    lib/libdlagg_tuning.so), unless the library there already carries this tree's build id."""
+    """Compile csrc/dlagg.hip and csrc/bound.hip for gfx950 (at the same time) into lib/libdlagg.so (in-tree;
+    tuning=True: the A/B build, lib/libdlagg_tuning.so), unless the library there already carries this tree's
+    build id."""
     out = os.path.join(PKG_ROOT, "lib", "libdlagg_tuning.so" if tuning else "libdlagg.so")
     bid = source_build_id(tuning)
     if not force and file_build_id(out) == bid:
@@ -133,12 +147,24 @@ def build(force: bool = False, verbose: bool = False, tuning: bool = False) -> s
     os.makedirs(os.path.dirname(out), exist_ok=True)
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     tmp = out + ".tmp"
-    cmd = [hipcc, *HIPCC_FLAGS, *(_TUNING_FLAGS if tuning else []), '-DDLA_BUILD_ID="%s"' % bid, "-I", INCLUDE,
-           "-o", tmp, CSRC]
+    common = [hipcc, *(f for f in HIPCC_FLAGS if f != "-shared"), *(_TUNING_FLAGS if tuning else []),
+              '-DDLA_BUILD_ID="%s"' % bid, "-I", INCLUDE, "-c"]
+    objects = [tmp + ".dlagg.o", tmp + ".bound.o"]
+    cmds = [common + ["-o", objects[0], CSRC], common + BOUND_FLAGS + ["-o", objects[1], CSRC_BOUND]]
+    link = [hipcc, "--offload-arch=gfx950", "-fPIC", "-shared", "-o", tmp, *objects]
     if verbose:
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
-    os.replace(tmp, out)
+        print("\n".join(" ".join(c) for c in cmds + [link]))
+    try:
+        running = [subprocess.Popen(c) for c in cmds]
+        for c, status in zip(cmds, [p.wait() for p in running]):
+            if status:
+                raise subprocess.CalledProcessError(status, c)
+        subprocess.run(link, check=True)
+        os.replace(tmp, out)
+    finally:
+        for path in objects:
+            if os.path.exists(path):
+                os.remove(path)
     return out
 
 
@@ -348,6 +374,27 @@ class _Lib:
         so.dla_wsum_mixed.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(vp),
                                       ctypes.POINTER(ctypes.c_double), ctypes.c_int, ctypes.c_int64, vp, vp]
         so.dla_wsum_mixed.restype = ctypes.c_int
+        i32p, i64p, vpp, dblp = (ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(vp),
+                                 ctypes.POINTER(ctypes.c_double))
+        so.dla_norm_workspace.argtypes = [ctypes.c_int]
+        so.dla_norm_workspace.restype = ctypes.c_int64
+        so.dla_norm.argtypes = [ctypes.c_int, i32p, vpp, i64p, ctypes.c_int, ctypes.c_int, vp, vp, ctypes.c_int64, vp]
+        so.dla_norm.restype = ctypes.c_int
+        so.dla_norm_scale.argtypes = [ctypes.c_int, i32p, vpp, vpp, i64p, ctypes.c_int, ctypes.c_double, ctypes.c_double,
+                                      ctypes.c_int, vp, vp, ctypes.c_int64, vp]
+        so.dla_norm_scale.restype = ctypes.c_int
+        so.dla_peer_workspace.argtypes = [ctypes.c_int, ctypes.c_int]
+        so.dla_peer_workspace.restype = ctypes.c_int64
+        so.dla_peer_norms.argtypes = [ctypes.c_int, i32p, vpp, vpp, i64p, ctypes.c_int, vp, ctypes.c_int, vp, vp,
+                                      ctypes.c_int64, vp]
+        so.dla_peer_norms.restype = ctypes.c_int
+        so.dla_wsum_bounded.argtypes = [ctypes.c_int, i32p, vpp, vpp, vpp, i64p, dblp, ctypes.c_int, ctypes.c_double, vp,
+                                        ctypes.c_int, vp, vp, ctypes.c_int64, vp]
+        so.dla_wsum_bounded.restype = ctypes.c_int
+        so.dla_wsum_bounded_slab_tiled.argtypes = [ctypes.c_int, vp, ctypes.c_int64, ctypes.c_int64, vp, dblp,
+                                                   ctypes.c_int, ctypes.c_int64, ctypes.c_double, vp, ctypes.c_int, vp,
+                                                   vp, ctypes.c_int64, vp]
+        so.dla_wsum_bounded_slab_tiled.restype = ctypes.c_int
         so.dla_plan_destroy.argtypes = [vp]
         so.dla_plan_destroy.restype = None
         v = so.dla_version()
@@ -444,6 +491,64 @@ def mean_ptrs(dtype_code: int, peer_ptrs: Sequence[int], n_elems: int, out_ptr: 
     L = lib()
     rc = L.so.dla_mean(dtype_code, _ptr_array(peer_ptrs), len(peer_ptrs), n_elems, out_ptr, stream_ptr)
     L.check(rc, "dla_mean")
+
+
+NORM_CODES = {2.0: 2, 1.0: 1, float("inf"): 0}  # DLA_NORM_*
+
+
+def norm_workspace(n_tensors: int) -> int:
+    """dla_norm_workspace: bytes of the workspace of norm_ptrs / norm_scale_ptrs."""
+    return int(lib().so.dla_norm_workspace(n_tensors))
+
+
+def norm_ptrs(n_tensors: int, codes, ptrs, numels, norm: int, out_code: int, out_ptr, ws_ptr: int, ws_bytes: int,
+              stream_ptr: int) -> None:
+    """dla_norm on ctypes tables (int dtypes, device pointers, int64 numels); out_ptr None: partial sums only."""
+    L = lib()
+    L.check(L.so.dla_norm(n_tensors, codes, ptrs, numels, norm, out_code, out_ptr, ws_ptr, ws_bytes, stream_ptr),
+            "dla_norm")
+
+
+def norm_scale_ptrs(n_tensors: int, codes, ptrs, out_ptrs, numels, norm: int, max_norm: float, eps: float, out_code: int,
+                    norm_ptr, ws_ptr: int, ws_bytes: int, stream_ptr: int) -> None:
+    """dla_norm_scale behind norm_ptrs of the same tables and workspace."""
+    L = lib()
+    L.check(L.so.dla_norm_scale(n_tensors, codes, ptrs, out_ptrs, numels, norm, max_norm, eps, out_code, norm_ptr, ws_ptr,
+                                ws_bytes, stream_ptr), "dla_norm_scale")
+
+
+def peer_workspace(n_tensors: int, n_peers: int) -> int:
+    """dla_peer_workspace: bytes of the workspace of peer_norms_ptrs / wsum_bounded_ptrs (0: out of range)."""
+    return int(lib().so.dla_peer_workspace(n_tensors, n_peers))
+
+
+def peer_norms_ptrs(n_tensors: int, codes, peer_ptrs, center_ptrs, numels, n_peers: int, sq_ptr, out_code: int, norms_ptr,
+                    ws_ptr: int, ws_bytes: int, stream_ptr: int) -> None:
+    """dla_peer_norms on ctypes tables (peer_ptrs tensor-major)."""
+    L = lib()
+    L.check(L.so.dla_peer_norms(n_tensors, codes, peer_ptrs, center_ptrs, numels, n_peers, sq_ptr, out_code, norms_ptr,
+                                ws_ptr, ws_bytes, stream_ptr), "dla_peer_norms")
+
+
+def wsum_bounded_ptrs(n_tensors: int, codes, peer_ptrs, center_ptrs, out_ptrs, numels, weights: Sequence[float],
+                      n_peers: int, max_norm: float, sq_ptr, out_code: int, norms_ptr, ws_ptr: int, ws_bytes: int,
+                      stream_ptr: int) -> None:
+    """dla_wsum_bounded on ctypes tables (peer_ptrs tensor-major)."""
+    L = lib()
+    _check_tables("wsum_bounded", n_peers, 1, weights=weights)
+    L.check(L.so.dla_wsum_bounded(n_tensors, codes, peer_ptrs, center_ptrs, out_ptrs, numels, _dbl_array(weights), n_peers,
+                                  max_norm, sq_ptr, out_code, norms_ptr, ws_ptr, ws_bytes, stream_ptr),
+            "dla_wsum_bounded")
+
+
+def wsum_bounded_slab_tiled_ptr(dtype_code: int, base_ptr: int, tile_elems: int, slab_rows: int, center_ptr,
+                                weights: Sequence[float], n_elems: int, max_norm: float, out_ptr: int, out_code: int,
+                                norms_ptr, ws_ptr: int, ws_bytes: int, stream_ptr: int) -> None:
+    """dla_wsum_bounded_slab_tiled over rows 0..len(weights)-1 (center_ptr None: row 0 is the centre)."""
+    L = lib()
+    L.check(L.so.dla_wsum_bounded_slab_tiled(dtype_code, base_ptr, tile_elems, slab_rows, center_ptr, _dbl_array(weights),
+                                             len(weights), n_elems, max_norm, out_ptr, out_code, norms_ptr, ws_ptr,
+                                             ws_bytes, stream_ptr), "dla_wsum_bounded_slab_tiled")
 
 
 def wsum_slab_ptr(dtype_code: int, base_ptr: int, pitch_elems: int, weights: Sequence[float], n_peers: int,

@@ -13,6 +13,7 @@ from torch import nn
 
 class GradientAggregationMethod(IntEnum):
     FEDAVG = 1
+    NORM_BOUNDED_FEDAVG = 2  # norm_bounded.NormBoundedFedAvg; the reference has no such method
 
 
 class GradientAggregation:

@@ -24,6 +24,7 @@ import torch.nn as nn
 from accdfl_amd.core.gradient_aggregation import GradientAggregationMethod
 from accdfl_amd.core import wire
 from accdfl_amd.core.gradient_aggregation.fedavg import FedAvg, _center_copy
+from accdfl_amd.core.gradient_aggregation.norm_bounded import NormBoundedFedAvg
 
 
 def _native_fingerprint(model: nn.Module) -> Optional[bytes]:
@@ -72,6 +73,10 @@ class ModelManager:
     def get_aggregation_method(self):
         if self.settings.gradient_aggregation == GradientAggregationMethod.FEDAVG:
             return FedAvg
+        if self.settings.gradient_aggregation == GradientAggregationMethod.NORM_BOUNDED_FEDAVG:
+            # updates are measured from the manager's own model (DFL's per-round managers have none: from the
+            # first model that arrived)
+            return NormBoundedFedAvg(self.settings.max_update_norm, center=self.model)
 
     def aggregate_trained_models(self, weights: List[float] = None) -> Optional[nn.Module]:
         models = [model for model in self.incoming_trained_models.values()]
@@ -330,8 +335,10 @@ class DeviceModelManager(ModelManager):
         return True
 
     def aggregate_trained_models(self, weights: List[float] = None) -> Optional[nn.Module]:
-        if self.get_aggregation_method() is not FedAvg or not self._uniform():
-            return self.get_aggregation_method().aggregate(self._modules(), weights=weights)
+        method = self.get_aggregation_method()
+        bounded = isinstance(method, NormBoundedFedAvg)
+        if not (method is FedAvg or bounded) or not self._uniform():
+            return method.aggregate(self._modules(), weights=weights)
         entries = list(self.incoming_trained_models.values())
         n = len(entries)
         if not weights:
@@ -349,7 +356,11 @@ class DeviceModelManager(ModelManager):
                         buf.copy_(first.state_dict[name])
             else:
                 center = _center_copy(first)  # deepcopy(models[0]) minus the parameter values
-            self.slab.reduce_into(list(center.parameters()), weights)
+            if bounded:
+                self.slab.reduce_bounded_into(list(center.parameters()), method.max_norm, weights,
+                                              center=None if method.center is None else list(method.center.parameters()))
+            else:
+                self.slab.reduce_into(list(center.parameters()), weights)
         return center
 
     def aggregate_serialized(self, weights: List[float] = None) -> bytes:

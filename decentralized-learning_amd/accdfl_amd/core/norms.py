@@ -1,0 +1,404 @@
+"""Norms over many tensors, and what is bounded by them (include/dlagg.h, csrc/bound.hip).
+
+A training step clips its gradient by the global norm over every parameter; a round bounds what one peer may move
+the average by.  The reference does neither (its trainer steps at accdfl/core/model_trainer.py:18-121, its
+aggregator averages whatever arrived, accdfl/core/gradient_aggregation/fedavg.py:20-25); both read every element
+of a model once before the first element can be written, which is what these operators are built around::
+
+    global_norm(tensors)                         one number over a list of tensors
+    clip_global_norm(tensors, max_norm)          the list scaled to at most that norm, into new or given tensors
+    clip_global_norm_(tensors, max_norm)         the same in place
+    clip_grad_norm_(parameters, max_norm)        the same on parameters' gradients (torch.nn.utils' contract)
+    update_norms(models, center)                 how far each model lies from a centre
+    wsum_bounded(peers, weights, center, R)      center + sum_k w_k min(1, R / n_k) (peer_k - center), flat peers
+    wsum_bounded_multi(...)                      the same over the tensors of whole models
+
+Tensors are float32 / bfloat16 / float16 / float64, mixed freely within a list, on one HIP device, empty ones
+included.  Dense tensors are read where they are whatever the order of their axes and wherever they start; others
+(a slice with gaps, an expanded tensor) are copied first.  Sums, norms and averages are carried in 64 bits and
+rounded once.  Results are on the device and nothing synchronises; nothing here is differentiable.  Work is
+enqueued on ``stream`` or the current stream of the tensors' device, workspaces come from torch's caching
+allocator for each call, and every launch takes its tables by value: calls on several streams or threads do not
+meet, and a call captured into a graph replays.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
+
+import torch
+from torch import nn
+
+from accdfl_amd import _lib
+from accdfl_amd.core import wsum as _wsum
+
+Tensors = Union[nn.Module, torch.Tensor, Iterable[torch.Tensor]]
+
+CLIP_EPS = 1e-6  # the norm is raised by this before the bound is divided by it (torch.nn.utils.clip_grad_norm_)
+MAX_PEERS = 2048  # include/dlagg.h dla_peer_workspace
+
+
+# ------------------------------------------------------------------------------------------- tables of tensors
+class _Tables:
+    """What one call hands to the library: dtype codes and counts of T tensors, the addresses of the first
+    ``lead`` lists, and those of the other lists tensor-major."""
+
+    __slots__ = ("n", "device", "codes", "numels", "lead", "rest", "wide")
+
+    def __init__(self, n, device, codes, numels, lead, rest, wide):
+        self.n = n
+        self.device = device
+        self.codes = codes
+        self.numels = numels
+        self.lead = lead
+        self.rest = rest
+        self.wide = wide  # float64 among the tensors
+
+    @property
+    def out_dtype(self) -> torch.dtype:
+        return torch.float64 if self.wide else torch.float32
+
+    @property
+    def out_code(self) -> int:
+        return _lib.DLA_F64 if self.wide else _lib.DLA_F32
+
+
+def _pack(lists: List[List[torch.Tensor]], lead: int, bump: int = -1) -> Optional[_Tables]:
+    """The tables of lists whose tensors the kernels take as they are (walk.cpp dense_lists), else None.
+    ``bump``: the list that the call writes (its tensors' version counters move on)."""
+    mod = _lib.walk_module()
+    if mod is None:
+        return None
+    r = mod.dense_lists(lists, lead, bump)
+    if r is None:
+        return None
+    device, codes, numels, head, tail, wide = r
+    n = len(lists[0])
+    row = ctypes.c_void_p * n
+    return _Tables(n, torch.device("cuda", device), (ctypes.c_int * n).from_buffer(codes),
+                   (ctypes.c_int64 * n).from_buffer(numels), [row.from_buffer(head, 8 * n * i) for i in range(lead)],
+                   (ctypes.c_void_p * (len(tail) // 8)).from_buffer(tail) if len(tail) else None, wide)
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Every element of the tensor's memory span is one element of the tensor (any order of its axes)."""
+    if t.numel() < 2:
+        return True
+    expect = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.stride() == b.stride() or (a.is_contiguous() and b.is_contiguous())
+
+
+def _check(lists: List[List[torch.Tensor]], names: Sequence[str]) -> torch.device:
+    """Raises for lists that no copy makes fit: types, devices, dtypes, counts, sizes."""
+    first = lists[0]
+    device = None
+    for name, ts in zip(names, lists):
+        if len(ts) != len(first):
+            raise ValueError("%s has %d tensors, %s has %d" % (name, len(ts), names[0], len(first)))
+        for i, t in enumerate(ts):
+            what = "%s tensor %d" % (name, i)
+            if not isinstance(t, torch.Tensor):
+                raise TypeError("%s is a %s, not a tensor" % (what, type(t).__name__))
+            if t.layout is not torch.strided:
+                raise TypeError("%s is %s: only dense (strided) tensors are supported" % (what, t.layout))
+            _wsum.dtype_code(t.dtype)
+            if device is None:
+                device = _wsum.require_device(t.device if t.is_cuda else None)
+            if t.device != device:
+                raise ValueError("%s is on %s, expected %s" % (what, t.device, device))
+            if t.dtype != first[i].dtype or t.shape != first[i].shape:
+                raise ValueError("%s is %s %s, %s has %s %s there" % (what, t.dtype, tuple(t.shape), names[0],
+                                                                      first[i].dtype, tuple(first[i].shape)))
+    return device
+
+
+def _pack_checked(lists: List[List[torch.Tensor]], names: Sequence[str], lead: int, out: int = -1):
+    """(tables, copies to write back) for any lists that _check accepts: tensors that are not dense, or whose
+    element order differs within their place, are replaced by contiguous copies; lists[out]'s replacements are
+    returned as (tensor, its copy) to be copied back after the call."""
+    device = _check(lists, names)
+    lists = [list(ts) for ts in lists]
+    back = []
+    if out >= 0:
+        for t in lists[out]:
+            if any(st == 0 and sz > 1 for st, sz in zip(t.stride(), t.shape)):
+                raise ValueError("an output has elements that share memory (an expanded tensor)")
+    for i in range(len(lists[0])):
+        place = [ts[i] for ts in lists]
+        if all(_dense(t) and not t.is_neg() and _same_order(t, place[0]) for t in place):
+            continue
+        for ts, t in zip(lists, place):
+            ts[i] = t.detach().resolve_neg().contiguous()
+        if out >= 0:
+            if lists[out][i].data_ptr() != place[out].data_ptr():
+                lists[out][i] = torch.empty(place[out].shape, dtype=place[out].dtype, device=device)
+                back.append((place[out], lists[out][i]))
+    tables = _pack(lists, lead, out)
+    if tables is None:
+        n, rest = len(lists[0]), lists[lead:]
+        row = ctypes.c_void_p * n
+        address = lambda t: t.data_ptr() if t.numel() else 0  # noqa: E731
+        tables = _Tables(n, device, (ctypes.c_int * n)(*[_wsum.dtype_code(t.dtype) for t in lists[0]]),
+                         (ctypes.c_int64 * n)(*[t.numel() for t in lists[0]]),
+                         [row(*[address(t) for t in ts]) for ts in lists[:lead]],
+                         (ctypes.c_void_p * (n * len(rest)))(*[address(ts[i]) for i in range(n) for ts in rest])
+                         if rest else None, any(t.dtype == torch.float64 for t in lists[0]))
+        if out >= 0:
+            torch.autograd.graph.increment_version([t for t in lists[out] if not t.is_inference()])
+    return tables, back, lists  # the lists keep the copies alive until the call is enqueued
+
+
+def _tensors_of(what: Tensors) -> List[torch.Tensor]:
+    if isinstance(what, torch.Tensor):
+        return [what]
+    if isinstance(what, nn.Module):
+        return list(what.parameters())
+    return what if type(what) is list else list(what)
+
+
+def _norm_code(norm_type: float) -> int:
+    code = _lib.NORM_CODES.get(float(norm_type))
+    if code is None:
+        raise ValueError("norm_type must be 1, 2 or inf, got %r" % (norm_type,))
+    return code
+
+
+def _bound(max_norm: float) -> float:
+    r = float(max_norm)
+    if not r >= 0.0:
+        raise ValueError("max_norm must be >= 0, got %r" % (max_norm,))
+    return r
+
+
+@contextlib.contextmanager
+def _placed(device: torch.device, stream: torch.cuda.Stream):
+    with torch.cuda.device(device), torch.cuda.stream(stream):
+        yield
+
+
+def _place(device: torch.device, stream: Optional[torch.cuda.Stream]):
+    """The device, and the stream when one is given, made current for a call: allocations and launches of the
+    call belong to them."""
+    if stream is None:
+        if device.index == torch.cuda.current_device():
+            return contextlib.nullcontext()
+        return torch.cuda.device(device)
+    if stream.device != device:
+        raise ValueError("stream is on %s, the tensors are on %s" % (stream.device, device))
+    return _placed(device, stream)
+
+
+def _raw_stream(device: torch.device) -> int:
+    return int(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _device_of(tensors: List[torch.Tensor], stream: Optional[torch.cuda.Stream]) -> torch.device:
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.is_cuda:
+            return t.device
+    return stream.device if stream is not None else _wsum.require_device(None)
+
+
+def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _refuse_nonfinite(norm: torch.Tensor, norm_type: float) -> None:
+    if not bool(torch.isfinite(norm)):
+        raise RuntimeError("the total norm of order %s is not finite, so it cannot be clipped by; pass "
+                           "error_if_nonfinite=False to scale by it anyway" % float(norm_type))
+
+
+def _refuse_capture() -> None:
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("error_if_nonfinite=True reads the norm on the host, which a captured call cannot")
+
+
+# --------------------------------------------------------------------------------- a list of tensors: the norm
+def global_norm(tensors: Tensors, norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """The norm of all elements of ``tensors`` (tensors, a module's parameters, or one tensor) as if they were one
+    vector: ``norm_type`` 2, 1 or inf.  A scalar on their device, float32 (float64 if any tensor is); 0 for no
+    elements.  NaN anywhere gives NaN; ``error_if_nonfinite`` then raises instead (it waits for the GPU)."""
+    code = _norm_code(norm_type)
+    tensors = _tensors_of(tensors)
+    with _place(_device_of(tensors, stream), stream):
+        if error_if_nonfinite:
+            _refuse_capture()
+        if not tensors:
+            return torch.zeros((), dtype=torch.float32, device=_device_of(tensors, stream))
+        tables, keep = _pack([tensors], 1), None
+        if tables is None:
+            tables, _, keep = _pack_checked([tensors], ["tensors"], 1)
+        out = torch.empty((), dtype=tables.out_dtype, device=tables.device)
+        nbytes = _lib.norm_workspace(tables.n)
+        ws = _workspace(nbytes, tables.device)
+        _lib.norm_ptrs(tables.n, tables.codes, tables.lead[0], tables.numels, code, tables.out_code, out.data_ptr(),
+                       ws.data_ptr(), nbytes, _raw_stream(tables.device))
+        del keep
+        if error_if_nonfinite:
+            _refuse_nonfinite(out, norm_type)
+        return out
+
+
+def clip_global_norm(tensors: Tensors, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                     outs: Optional[Sequence[torch.Tensor]] = None,
+                     stream: Optional[torch.cuda.Stream] = None) -> Tuple[List[torch.Tensor], torch.Tensor]:
+    """(``tensors`` times ``min(1, max_norm / (norm + 1e-6))``, their norm): what a list of tensors becomes under a
+    largest global norm, the products rounded once to each tensor's dtype.  ``outs``: tensors of the same sizes
+    and dtypes to write (``outs[i]`` may be ``tensors[i]``; no other overlap), else new ones.  A NaN norm makes
+    everything NaN and an infinite one multiplies by 0, as torch.nn.utils.clip_grad_norm_ does;
+    ``error_if_nonfinite`` raises before anything is written instead (it waits for the GPU)."""
+    code = _norm_code(norm_type)
+    bound = _bound(max_norm)
+    tensors = _tensors_of(tensors)
+    with _place(_device_of(tensors, stream), stream), torch.no_grad():
+        if error_if_nonfinite:
+            _refuse_capture()
+        if outs is None:
+            outs = [torch.empty_like(t, requires_grad=False) if isinstance(t, torch.Tensor) else t for t in tensors]
+        else:
+            outs = _tensors_of(outs)
+        if len(outs) != len(tensors):
+            raise ValueError("clip_global_norm: %d outs for %d tensors" % (len(outs), len(tensors)))
+        if not tensors:
+            return list(outs), torch.zeros((), dtype=torch.float32, device=_device_of(tensors, stream))
+        tables, back, keep = _pack([tensors, outs], 2, bump=1), (), None
+        if tables is None:
+            tables, back, keep = _pack_checked([tensors, outs], ["tensors", "outs"], 2, out=1)
+        norm = torch.empty((), dtype=tables.out_dtype, device=tables.device)
+        nbytes = _lib.norm_workspace(tables.n)
+        ws = _workspace(nbytes, tables.device)
+        raw = _raw_stream(tables.device)
+        _lib.norm_ptrs(tables.n, tables.codes, tables.lead[0], tables.numels, code, tables.out_code,
+                       norm.data_ptr() if error_if_nonfinite else None, ws.data_ptr(), nbytes, raw)
+        if error_if_nonfinite:
+            _refuse_nonfinite(norm, norm_type)
+        _lib.norm_scale_ptrs(tables.n, tables.codes, tables.lead[0], tables.lead[1], tables.numels, code, bound, CLIP_EPS,
+                             tables.out_code, norm.data_ptr(), ws.data_ptr(), nbytes, raw)
+        for t, copy in back:
+            t.copy_(copy)
+        del keep
+        return list(outs), norm
+
+
+def clip_global_norm_(tensors: Tensors, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                      stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """clip_global_norm in place; returns the norm before it.  Tensors that overlap are refused."""
+    tensors = _tensors_of(tensors)
+    return clip_global_norm(tensors, max_norm, norm_type, error_if_nonfinite, outs=tensors, stream=stream)[1]
+
+
+def clip_grad_norm_(parameters: Tensors, max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """torch.nn.utils.clip_grad_norm_'s contract: the gradients of ``parameters`` (parameters, or a module) clipped
+    in place by their global norm, which is returned.  Parameters without a gradient are skipped."""
+    grads = [p.grad for p in _tensors_of(parameters)]
+    return clip_global_norm_([g for g in grads if g is not None], max_norm, norm_type, error_if_nonfinite)
+
+
+# ----------------------------------------------------------------------------------------- peers around a centre
+def _pack_round(lists: List[List[torch.Tensor]], names, lead: int, out: int = -1):
+    tables = _pack(lists, lead, bump=out)
+    if tables is not None:
+        return tables, (), None
+    return _pack_checked(lists, names() if callable(names) else names, lead, out=out)
+
+
+def _check_peers(n: int) -> None:
+    if n < 1:
+        raise IndexError("list index out of range")
+    if n > MAX_PEERS:
+        raise ValueError("%d peers: at most %d in one call" % (n, MAX_PEERS))
+
+
+def update_norms(models: Sequence[Tensors], center: Tensors, stream: Optional[torch.cuda.Stream] = None,
+                 squared: bool = False) -> torch.Tensor:
+    """``|| model_k - center ||_2`` over all tensors of each model (lists of tensors, modules' parameters, or flat
+    tensors, all with the centre's sizes and dtypes): [len(models)], float32 (float64 if any tensor is).
+    ``squared``: the float64 squares instead, which ranks that hold one bucket of every model each add up."""
+    lists = [_tensors_of(center)] + [_tensors_of(m) for m in models]
+    n = len(lists) - 1
+    _check_peers(n)
+    device = _device_of(lists[0], stream)
+    with _place(device, stream):
+        if not lists[0] and not any(lists):
+            return torch.zeros(n, dtype=torch.float64 if squared else torch.float32, device=device)
+        tables, _, keep = _pack_round(lists, lambda: ["center"] + ["model %d" % k for k in range(n)], 1)
+        out = torch.empty(n, dtype=torch.float64 if squared else tables.out_dtype, device=tables.device)
+        nbytes = _lib.peer_workspace(tables.n, n)
+        ws = _workspace(nbytes, tables.device)
+        _lib.peer_norms_ptrs(tables.n, tables.codes, tables.rest, tables.lead[0], tables.numels, n,
+                             out.data_ptr() if squared else None, tables.out_code, None if squared else out.data_ptr(),
+                             ws.data_ptr(), nbytes, _raw_stream(tables.device))
+        del keep
+        return out
+
+
+def wsum_bounded_tables(tables: _Tables, outs, weights: Sequence[float], n: int, max_norm: float,
+                        sq_norms: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dla_wsum_bounded on packed tables (``tables.lead[0]`` the centre, ``tables.rest`` the peers, ``outs`` a
+    ctypes array of addresses) on the current stream; returns the update norms [n]."""
+    norms = torch.empty(n, dtype=tables.out_dtype, device=tables.device)
+    nbytes = _lib.peer_workspace(tables.n, n)
+    ws = _workspace(nbytes, tables.device)
+    _lib.wsum_bounded_ptrs(tables.n, tables.codes, tables.rest, tables.lead[0], outs, tables.numels, weights, n, max_norm,
+                           None if sq_norms is None else sq_norms.data_ptr(), tables.out_code, norms.data_ptr(),
+                           ws.data_ptr(), nbytes, _raw_stream(tables.device))
+    return norms
+
+
+def wsum_bounded_multi(peer_params: Sequence[Tensors], weights: Sequence[float], center_params: Tensors, max_norm: float,
+                       outs: Sequence[torch.Tensor], stream: Optional[torch.cuda.Stream] = None,
+                       sq_norms: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The average of norm-bounded updates over the tensors of whole models::
+
+        n_k     = || peer_k - center ||_2  over all its tensors
+        outs[i] = center[i] + sum_k weights[k] * min(1, max_norm / n_k) * (peer_k[i] - center[i])
+
+    in list order, carried in 64 bits and rounded once.  A peer whose update is not finite (n_k is NaN or infinite)
+    adds nothing.  ``outs[i]`` may be the i-th tensor of the centre or of a peer; no other overlap.  ``sq_norms``:
+    float64 squared norms [n] on the device to bound by, when the tensors are one bucket of models whose norms are
+    known (update_norms(squared=True), added up).  Returns the norms [n], float32 (float64 if any tensor is)."""
+    bound = _bound(max_norm)
+    outs = _tensors_of(outs)
+    lists = [_tensors_of(center_params), outs] + [_tensors_of(p) for p in peer_params]
+    n = len(lists) - 2
+    _check_peers(n)
+    if len(weights) != n:
+        raise AssertionError("len(weights) != len(peers)")
+    device = _device_of(lists[0], stream)
+    with _place(device, stream), torch.no_grad():
+        if not any(lists):
+            return torch.zeros(n, dtype=torch.float32, device=device) if sq_norms is None else sq_norms.sqrt().float()
+        tables, back, keep = _pack_round(lists, lambda: ["center", "outs"] + ["peer %d" % k for k in range(n)], 2, out=1)
+        if sq_norms is not None and (sq_norms.dtype != torch.float64 or sq_norms.numel() != n
+                                     or sq_norms.device != tables.device or not sq_norms.is_contiguous()):
+            raise ValueError("sq_norms must be %d contiguous float64 values on %s" % (n, tables.device))
+        norms = wsum_bounded_tables(tables, tables.lead[1], weights, n, bound, sq_norms)
+        for t, copy in back:
+            t.copy_(copy)
+        del keep
+        return norms
+
+
+def wsum_bounded(peers: Sequence[torch.Tensor], weights: Sequence[float], center: torch.Tensor, max_norm: float,
+                 out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None,
+                 sq_norms: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """wsum_bounded_multi of one buffer per peer (wsum's flat peers): (the bounded average, the norms).  ``out``
+    may be the centre or a peer.  With one peer of weight 1 it is that model pulled back to within ``max_norm`` of
+    the centre: what a client that bounds its own update sends."""
+    max_norm = _bound(max_norm)
+    if out is None:
+        with _place(_device_of([center], stream), stream):
+            out = torch.empty_like(center, requires_grad=False)
+    return out, wsum_bounded_multi([[p] for p in peers], weights, [center], max_norm, [out], stream, sq_norms)

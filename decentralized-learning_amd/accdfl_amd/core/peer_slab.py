@@ -332,7 +332,77 @@ class PeerSlab:
 
     def reduce_into(self, params: Sequence[torch.Tensor], weights: Optional[Sequence[float]] = None) -> None:
         """Reduce and write the result into ``params`` (CPU or device tensors)."""
-        flat = self._reduce_planned(weights)
+        self._write_into(params, self._reduce_planned(weights))
+
+    # ----------------------------------------------------------- norm-bounded reduce
+    def _center_row(self, center) -> torch.Tensor:
+        """A centre — the slab's flat layout on the device, or tensors of the slab's layout anywhere — as a flat
+        device vector of ``total`` elements."""
+        if isinstance(center, torch.Tensor):
+            if (center.dtype != self.dtype or center.numel() != self.total or center.device != self.device
+                    or not center.is_contiguous()):
+                raise ValueError("center must be a contiguous %s tensor of %d elements on %s"
+                                 % (self.dtype, self.total, self.device))
+            return center.detach().view(-1)
+        center = list(center)
+        if not self.matches(center):
+            raise ValueError("PeerSlab: the centre's parameter layout differs from the slab's")
+        if not center:
+            return torch.empty(0, dtype=self.dtype, device=self.device)
+        row = torch.cat([p.detach().reshape(-1) for p in center]) if len({p.device for p in center}) == 1 else (
+            torch.cat([p.detach().reshape(-1).to(self.device) for p in center]))
+        return row.to(self.device)
+
+    def reduce_bounded(self, max_norm: float, weights: Optional[Sequence[float]] = None, center=None,
+                       out: Optional[torch.Tensor] = None):
+        """(the average of norm-bounded updates over the staged rows, the update norms [n]) — norms.wsum_bounded_multi
+        in arrival order.  ``center``: a flat device vector, tensors of the slab's layout (CPU or device), or
+        None: row 0, the first model that arrived."""
+        from accdfl_amd.core import norms as _norms
+
+        n = self.n
+        if not weights:
+            weights = [float(1. / n) for _ in range(n)]
+        else:
+            assert len(weights) == n
+        bound = _norms._bound(max_norm)
+        _norms._check_peers(n)
+        with _norms._place(self.device, None), torch.no_grad():
+            cur = torch.cuda.current_stream(self.device)
+            cur.wait_stream(self.copy_stream)
+            if out is None:
+                out = torch.empty(self.total, dtype=self.dtype, device=self.device)
+            if out.device != self.device or out.dtype != self.dtype or out.numel() < self.total or not out.is_contiguous():
+                raise ValueError("out must be a contiguous %s tensor of >= %d elements on %s"
+                                 % (self.dtype, self.total, self.device))
+            row = None if center is None else self._center_row(center)
+            if self.layout == "rows":
+                rows = [self.buf[k, : self.total] for k in range(n)]
+                _, norms = _norms.wsum_bounded(rows, weights, rows[0] if row is None else row, bound,
+                                               out=out.view(-1)[: self.total])
+                return out, norms
+            wide = self.dtype == torch.float64
+            norms = torch.empty(n, dtype=torch.float64 if wide else torch.float32, device=self.device)
+            nbytes = _lib.peer_workspace(1, n)
+            ws = _norms._workspace(nbytes, self.device)
+            _lib.wsum_bounded_slab_tiled_ptr(self.code, self.buf.data_ptr(), self.tile, self.capacity,
+                                             None if row is None else row.data_ptr(), weights, self.total, bound,
+                                             out.data_ptr(), _lib.DLA_F64 if wide else _lib.DLA_F32, norms.data_ptr(),
+                                             ws.data_ptr(), nbytes, int(cur.cuda_stream))
+        return out, norms
+
+    def reduce_bounded_into(self, params: Sequence[torch.Tensor], max_norm: float,
+                            weights: Optional[Sequence[float]] = None, center=None) -> torch.Tensor:
+        """reduce_bounded written into ``params`` (CPU or device tensors); returns the update norms."""
+        if self._flat is None:
+            self._flat = torch.empty(self.pitch, dtype=self.dtype, device=self.device)
+        flat, norms = self.reduce_bounded(max_norm, weights, center, out=self._flat)
+        self._write_into(params, flat[: self.total])
+        return norms
+
+    def _write_into(self, params: Sequence[torch.Tensor], flat: torch.Tensor) -> None:
+        """The flat result into ``params``: device tensors by copies in stream order, CPU tensors complete when
+        this returns."""
         if all(p.device == self.device for p in params):
             for p, v in zip(params, self.unflatten(flat)):
                 p.copy_(v)

@@ -57,7 +57,10 @@ class BucketShardedFedAvg:
     """FedAvg of an ``n_elems``-element flat model over the ranks of ``group``."""
 
     def __init__(self, n_elems: int, dtype: torch.dtype, group: Optional[dist.ProcessGroup] = None,
-                 device: Optional[torch.device] = None, reducer: Optional[Reducer] = None):
+                 device: Optional[torch.device] = None, reducer: Optional[Reducer] = None, bounded=None):
+        """``reducer`` / ``bounded``: replacements of the HIP kernels — of reduce_bucket, and of
+        reduce_bucket_bounded as the pair (squared norms of (peers, center), average of (peers, weights, center,
+        max_norm, squared norms, out)) — which the CPU tests give."""
         self.group = group
         self.rank = dist.get_rank(group) if dist.is_initialized() else 0
         self.world = dist.get_world_size(group) if dist.is_initialized() else 1
@@ -69,6 +72,7 @@ class BucketShardedFedAvg:
         start, end = self.bounds[0]
         self.bucket_len = end - start  # every bucket is padded to this length for the collectives
         self.reducer = reducer if reducer is not None else _hip_reducer
+        self.bounded = bounded
 
     @property
     def local_range(self) -> Tuple[int, int]:
@@ -88,6 +92,52 @@ class BucketShardedFedAvg:
             out = torch.zeros(self.bucket_len, dtype=self.dtype, device=self.device)
         if m > 0:
             self.reducer([p[:m] for p in peer_buckets], weights, out[:m])
+        return out
+
+    def update_sq_norms(self, peer_buckets: Sequence[torch.Tensor], center_bucket: torch.Tensor) -> torch.Tensor:
+        """float64 squared norms of the peers' updates over the WHOLE model: this rank's bucket of every peer
+        against its bucket of the centre (norms.update_norms), added up over the ranks by one all-reduce of
+        n_peers values."""
+        start, end = self.local_range
+        m = end - start
+        if self.bounded is not None:
+            sq = self.bounded[0]([p[:m] for p in peer_buckets], center_bucket[:m])
+        else:
+            from accdfl_amd.core import norms as _norms
+
+            sq = _norms.update_norms([[p[:m]] for p in peer_buckets], [center_bucket[:m]], squared=True)
+        if self.world > 1:
+            if sq.is_cuda and dist.get_backend(self.group) == "gloo":  # gloo takes CPU tensors
+                host = sq.cpu()
+                dist.all_reduce(host, group=self.group)
+                sq = host.to(sq.device)
+            else:
+                dist.all_reduce(sq, group=self.group)
+        return sq
+
+    def reduce_bucket_bounded(self, peer_buckets: Sequence[torch.Tensor], center_bucket: torch.Tensor, max_norm: float,
+                              weights: Optional[Sequence[float]] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """reduce_bucket with every peer's update bounded by its norm over the whole model
+        (norms.wsum_bounded): this rank's bucket, padded to ``bucket_len``.  Collective: every rank calls it, ranks
+        with an empty bucket too."""
+        n = len(peer_buckets)
+        if not weights:
+            weights = [float(1. / n) for _ in range(n)]
+        else:
+            assert len(weights) == n
+        start, end = self.local_range
+        m = end - start
+        sq = self.update_sq_norms(peer_buckets, center_bucket)
+        if out is None:
+            out = torch.zeros(self.bucket_len, dtype=self.dtype, device=self.device)
+        if m > 0:
+            peers, center = [p[:m] for p in peer_buckets], center_bucket[:m]
+            if self.bounded is not None:
+                self.bounded[1](peers, weights, center, max_norm, sq, out[:m])
+            else:
+                from accdfl_amd.core import norms as _norms
+
+                _norms.wsum_bounded(peers, weights, center, max_norm, out=out[:m], sq_norms=sq)
         return out
 
     def all_gather(self, bucket_out: torch.Tensor, full: Optional[torch.Tensor] = None) -> torch.Tensor:

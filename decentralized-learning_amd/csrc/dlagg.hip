@@ -55,8 +55,9 @@
 #include <unistd.h>
 
 #include "dlagg.h"
+#include "dlagg_internal.h"
 
-// Hash of this file, include/dlagg.h and the compile flags, set by the build
+// Hash of the library's sources, include/dlagg.h and the compile flags, set by the build
 // (accdfl_amd/_lib.py build()); the loader refuses a library whose id differs from the tree's.
 #ifndef DLA_BUILD_ID
 #define DLA_BUILD_ID "unversioned"
@@ -2508,6 +2509,9 @@ struct dla_plan {
   dla_launch_cfg_t cfg;
   bool has_cfg;
 };
+
+int dla_internal_fail(int code, const char* msg) { return fail(code, msg); }
+void dla_internal_clear_error() { g_last_error.clear(); }
 
 extern "C" {
 

@@ -224,6 +224,68 @@ int dla_wsum_mixed(int out_dtype, const int* peer_dtypes, const void* const* pee
  * peers[0] (also when n_peers > DLA_MAX_PEERS_PER_PASS). */
 int dla_mean(int dtype, const void* const* peers, int n_peers, int64_t n_elems, void* out, void* stream);
 
+/* ---- norms over many tensors, and what is bounded by them (additive in ABI v13) ----
+ *
+ * Tensors are dense and of any of the four dtypes, mixed freely within a call; their pointers need element
+ * alignment only.  Sums and norms are carried in 64 bits.  Nothing synchronises; the stream's device must be
+ * current.  Launches take everything by value except the caller's buffers, so a captured call replays.  The
+ * workspaces are the caller's, need no initialisation and hold nothing between calls (dla_norm's partial sums
+ * until the dla_norm_scale behind it has run); two calls in flight at once need two. */
+#define DLA_NORM_INF 0
+#define DLA_NORM_L1 1
+#define DLA_NORM_L2 2
+
+/* Bytes of the workspace of dla_norm / dla_norm_scale over n_tensors tensors. */
+int64_t dla_norm_workspace(int n_tensors);
+
+/* The norm of all elements of n_tensors tensors together: sqrt(sum x^2), sum |x| or max |x| (0 for no elements;
+ * a NaN anywhere gives NaN), what a training step needs before it clips a model's gradient (the reference
+ * trains at accdfl/core/model_trainer.py:18-121 and does not clip).
+ *   dtypes, tensors, numels  host arrays of n_tensors
+ *   out        DEVICE pointer to one value of out_dtype (F32 or F64), or NULL: the partial sums only, for
+ *              dla_norm_scale
+ *   workspace  DEVICE memory of dla_norm_workspace(n_tensors) bytes, 8-byte aligned */
+int dla_norm(int n_tensors, const int* dtypes, const void* const* tensors, const int64_t* numels, int norm, int out_dtype,
+             void* out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* outs[t] = round(tensors[t] * min(1, max_norm / (n + eps))), n the norm whose partial sums dla_norm left in
+ * `workspace` for the same tensors, counts and norm earlier on this stream.  NaN norms make everything NaN,
+ * infinite ones give a factor of 0.  outs[t] may be tensors[t]; every other overlap is refused (DLA_E_ALIAS).  In
+ * place nothing is written when the factor is 1.  norm_out (F32 or F64, DEVICE) may be NULL. */
+int dla_norm_scale(int n_tensors, const int* dtypes, const void* const* tensors, void* const* outs, const int64_t* numels,
+                   int norm, double max_norm, double eps, int out_dtype, void* norm_out, const void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/* Bytes of the workspace of dla_peer_norms / dla_wsum_bounded(_slab_tiled, one tensor); 0 for arguments out of
+ * range (1 <= n_peers <= 2048). */
+int64_t dla_peer_workspace(int n_tensors, int n_peers);
+
+/* How far each of n_peers models lies from a centre: norms[k] = || p_k - c ||_2 over all tensors together.
+ *   peer_ptrs  host array [n_tensors * n_peers] of DEVICE pointers, tensor-major as dla_wsum_multi takes them
+ *   centers    host array [n_tensors]; tensor t of every peer and of the centre has dtypes[t] and numels[t]
+ *   sq_out     DEVICE doubles [n_peers], the squares (what ranks that hold one bucket each add up), or NULL
+ *   norms      DEVICE [n_peers] of out_dtype (F32 or F64), or NULL */
+int dla_peer_norms(int n_tensors, const int* dtypes, const void* const* peer_ptrs, const void* const* centers,
+                   const int64_t* numels, int n_peers, double* sq_out, int out_dtype, void* norms, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/* fedavg.py:20-25 with every peer's update bounded first:
+ *     out = round(c + sum_k a_k (p_k - c)),   a_k = weights[k] * (n_k <= max_norm ? 1 : max_norm / n_k)
+ * with n_k as dla_peer_norms gives it, in list order, carried in 64 bits and rounded once (dla_wsum rounds every
+ * step, as the reference does).  A peer whose n_k is not finite adds nothing and is not read.  outs[t] may be
+ * tensor t of the centre or of a peer; every other overlap is refused (DLA_E_ALIAS).
+ *   sq  DEVICE doubles [n_peers], the squared norms to bound by (a bucket of a model whose norms are known), or
+ *       NULL: computed here */
+int dla_wsum_bounded(int n_tensors, const int* dtypes, const void* const* peer_ptrs, const void* const* centers,
+                     void* const* outs, const int64_t* numels, const double* weights, int n_peers, double max_norm,
+                     const double* sq, int out_dtype, void* norms, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* dla_wsum_bounded over rows 0..n_peers-1 of a tile-interleaved slab (the layout of dla_wsum_slab_tiled; any
+ * dtype) into the contiguous `out`.  center: a contiguous DEVICE vector (out may be it), or NULL: row 0. */
+int dla_wsum_bounded_slab_tiled(int dtype, const void* base, int64_t tile_elems, int64_t slab_rows, const void* center,
+                                const double* weights, int n_peers, int64_t n_elems, double max_norm, void* out,
+                                int out_dtype, void* norms, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Largest peer count one kernel pass takes (kernel-argument pointer table). */
 int dla_max_peers_per_pass(void);
 
