@@ -92,8 +92,9 @@ EXPORTED = (
     "dla_wsum_mixed",
     "dla_norm_workspace",
     "dla_norm",
-    "dla_norm_scale",
+    "dla_norm_clip",
     "dla_peer_workspace",
+    "dla_peer_table",
     "dla_peer_norms",
     "dla_wsum_bounded",
     "dla_wsum_bounded_slab_tiled",
@@ -374,27 +375,24 @@ class _Lib:
         so.dla_wsum_mixed.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(vp),
                                       ctypes.POINTER(ctypes.c_double), ctypes.c_int, ctypes.c_int64, vp, vp]
         so.dla_wsum_mixed.restype = ctypes.c_int
-        i32p, i64p, vpp, dblp = (ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(vp),
-                                 ctypes.POINTER(ctypes.c_double))
-        so.dla_norm_workspace.argtypes = [ctypes.c_int]
-        so.dla_norm_workspace.restype = ctypes.c_int64
-        so.dla_norm.argtypes = [ctypes.c_int, i32p, vpp, i64p, ctypes.c_int, ctypes.c_int, vp, vp, ctypes.c_int64, vp]
-        so.dla_norm.restype = ctypes.c_int
-        so.dla_norm_scale.argtypes = [ctypes.c_int, i32p, vpp, vpp, i64p, ctypes.c_int, ctypes.c_double, ctypes.c_double,
-                                      ctypes.c_int, vp, vp, ctypes.c_int64, vp]
-        so.dla_norm_scale.restype = ctypes.c_int
-        so.dla_peer_workspace.argtypes = [ctypes.c_int, ctypes.c_int]
-        so.dla_peer_workspace.restype = ctypes.c_int64
-        so.dla_peer_norms.argtypes = [ctypes.c_int, i32p, vpp, vpp, i64p, ctypes.c_int, vp, ctypes.c_int, vp, vp,
-                                      ctypes.c_int64, vp]
-        so.dla_peer_norms.restype = ctypes.c_int
-        so.dla_wsum_bounded.argtypes = [ctypes.c_int, i32p, vpp, vpp, vpp, i64p, dblp, ctypes.c_int, ctypes.c_double, vp,
-                                        ctypes.c_int, vp, vp, ctypes.c_int64, vp]
-        so.dla_wsum_bounded.restype = ctypes.c_int
-        so.dla_wsum_bounded_slab_tiled.argtypes = [ctypes.c_int, vp, ctypes.c_int64, ctypes.c_int64, vp, dblp,
-                                                   ctypes.c_int, ctypes.c_int64, ctypes.c_double, vp, ctypes.c_int, vp,
-                                                   vp, ctypes.c_int64, vp]
-        so.dla_wsum_bounded_slab_tiled.restype = ctypes.c_int
+        # norms and norm bounds: their tables are passed as addresses
+        i32, i64, dbl = ctypes.c_int, ctypes.c_int64, ctypes.c_double
+        so.dla_norm_workspace.argtypes = [i32]
+        so.dla_norm_workspace.restype = i64
+        so.dla_norm.argtypes = [i32, vp, vp, vp, i32, i32, vp, vp, vp, i64, vp]
+        so.dla_norm.restype = i32
+        so.dla_norm_clip.argtypes = [i32, vp, vp, vp, vp, i32, dbl, dbl, i32, vp, vp, vp, i64, vp]
+        so.dla_norm_clip.restype = i32
+        so.dla_peer_workspace.argtypes = [i32, i32]
+        so.dla_peer_workspace.restype = i64
+        so.dla_peer_table.argtypes = [i32, i32]
+        so.dla_peer_table.restype = i64
+        so.dla_peer_norms.argtypes = [i32, vp, vp, vp, vp, i32, vp, i32, vp, vp, vp, i64, vp, i64, vp]
+        so.dla_peer_norms.restype = i32
+        so.dla_wsum_bounded.argtypes = [i32, vp, vp, vp, vp, vp, vp, i32, dbl, vp, i32, vp, vp, vp, i64, vp, i64, vp]
+        so.dla_wsum_bounded.restype = i32
+        so.dla_wsum_bounded_slab_tiled.argtypes = [i32, vp, i64, i64, vp, vp, i32, i64, dbl, vp, i32, vp, vp, vp, i64, vp]
+        so.dla_wsum_bounded_slab_tiled.restype = i32
         so.dla_plan_destroy.argtypes = [vp]
         so.dla_plan_destroy.restype = None
         v = so.dla_version()
@@ -448,10 +446,7 @@ def _ptr_array(ptrs: Sequence[int]):
 
 
 def _dbl_array(vals: Sequence[float]):
-    arr = (ctypes.c_double * len(vals))()
-    for i, v in enumerate(vals):
-        arr[i] = float(v)
-    return arr
+    return (ctypes.c_double * len(vals))(*[float(v) for v in vals])
 
 
 def wsum_ptrs(dtype_code: int, peer_ptrs: Sequence[int], weights: Sequence[float], n_elems: int, out_ptr: int,
@@ -494,61 +489,72 @@ def mean_ptrs(dtype_code: int, peer_ptrs: Sequence[int], n_elems: int, out_ptr: 
 
 
 NORM_CODES = {2.0: 2, 1.0: 1, float("inf"): 0}  # DLA_NORM_*
+COUNTER_BYTES = 65536  # DLA_COUNTER_BYTES
+
+# The norm entry points take their tables (dtype codes, device pointers, counts) as addresses.
 
 
 def norm_workspace(n_tensors: int) -> int:
-    """dla_norm_workspace: bytes of the workspace of norm_ptrs / norm_scale_ptrs."""
-    return int(lib().so.dla_norm_workspace(n_tensors))
+    """dla_norm_workspace: bytes of the workspace of norm_ptrs / norm_clip_ptrs."""
+    return lib().so.dla_norm_workspace(n_tensors)
 
 
-def norm_ptrs(n_tensors: int, codes, ptrs, numels, norm: int, out_code: int, out_ptr, ws_ptr: int, ws_bytes: int,
-              stream_ptr: int) -> None:
-    """dla_norm on ctypes tables (int dtypes, device pointers, int64 numels); out_ptr None: partial sums only."""
+def norm_ptrs(*args) -> None:
+    """dla_norm(n_tensors, dtypes, tensors, numels, norm, out_dtype, out, counter, workspace, bytes, stream)."""
     L = lib()
-    L.check(L.so.dla_norm(n_tensors, codes, ptrs, numels, norm, out_code, out_ptr, ws_ptr, ws_bytes, stream_ptr),
-            "dla_norm")
+    rc = L.so.dla_norm(*args)
+    if rc:
+        L.check(rc, "dla_norm")
 
 
-def norm_scale_ptrs(n_tensors: int, codes, ptrs, out_ptrs, numels, norm: int, max_norm: float, eps: float, out_code: int,
-                    norm_ptr, ws_ptr: int, ws_bytes: int, stream_ptr: int) -> None:
-    """dla_norm_scale behind norm_ptrs of the same tables and workspace."""
+def norm_clip_ptrs(*args) -> None:
+    """dla_norm_clip(n_tensors, dtypes, tensors, outs, numels, norm, max_norm, eps, out_dtype, norm_out, counter,
+    workspace, bytes, stream)."""
     L = lib()
-    L.check(L.so.dla_norm_scale(n_tensors, codes, ptrs, out_ptrs, numels, norm, max_norm, eps, out_code, norm_ptr, ws_ptr,
-                                ws_bytes, stream_ptr), "dla_norm_scale")
+    rc = L.so.dla_norm_clip(*args)
+    if rc:
+        L.check(rc, "dla_norm_clip")
 
 
 def peer_workspace(n_tensors: int, n_peers: int) -> int:
     """dla_peer_workspace: bytes of the workspace of peer_norms_ptrs / wsum_bounded_ptrs (0: out of range)."""
-    return int(lib().so.dla_peer_workspace(n_tensors, n_peers))
+    return lib().so.dla_peer_workspace(n_tensors, n_peers)
 
 
-def peer_norms_ptrs(n_tensors: int, codes, peer_ptrs, center_ptrs, numels, n_peers: int, sq_ptr, out_code: int, norms_ptr,
-                    ws_ptr: int, ws_bytes: int, stream_ptr: int) -> None:
-    """dla_peer_norms on ctypes tables (peer_ptrs tensor-major)."""
+def peer_table(n_tensors: int, n_peers: int) -> int:
+    """dla_peer_table: bytes of page-locked memory a call of this size is faster with (0: none)."""
+    return lib().so.dla_peer_table(n_tensors, n_peers)
+
+
+def peer_norms_ptrs(*args) -> None:
+    """dla_peer_norms(n_tensors, dtypes, peers, centers, numels, n_peers, sq, out_dtype, norms, counters, table_host,
+    table_bytes, workspace, bytes, stream)."""
     L = lib()
-    L.check(L.so.dla_peer_norms(n_tensors, codes, peer_ptrs, center_ptrs, numels, n_peers, sq_ptr, out_code, norms_ptr,
-                                ws_ptr, ws_bytes, stream_ptr), "dla_peer_norms")
+    rc = L.so.dla_peer_norms(*args)
+    if rc:
+        L.check(rc, "dla_peer_norms")
 
 
-def wsum_bounded_ptrs(n_tensors: int, codes, peer_ptrs, center_ptrs, out_ptrs, numels, weights: Sequence[float],
-                      n_peers: int, max_norm: float, sq_ptr, out_code: int, norms_ptr, ws_ptr: int, ws_bytes: int,
-                      stream_ptr: int) -> None:
-    """dla_wsum_bounded on ctypes tables (peer_ptrs tensor-major)."""
+def wsum_bounded_ptrs(n_tensors: int, codes, peers, centers, outs, numels, weights: Sequence[float], n_peers: int,
+                      *args) -> None:
+    """dla_wsum_bounded(n_tensors, dtypes, peers, centers, outs, numels, weights, n_peers, max_norm, sq, out_dtype,
+    norms, counters, table_host, table_bytes, workspace, bytes, stream)."""
     L = lib()
     _check_tables("wsum_bounded", n_peers, 1, weights=weights)
-    L.check(L.so.dla_wsum_bounded(n_tensors, codes, peer_ptrs, center_ptrs, out_ptrs, numels, _dbl_array(weights), n_peers,
-                                  max_norm, sq_ptr, out_code, norms_ptr, ws_ptr, ws_bytes, stream_ptr),
-            "dla_wsum_bounded")
+    rc = L.so.dla_wsum_bounded(n_tensors, codes, peers, centers, outs, numels, _dbl_array(weights), n_peers, *args)
+    if rc:
+        L.check(rc, "dla_wsum_bounded")
 
 
 def wsum_bounded_slab_tiled_ptr(dtype_code: int, base_ptr: int, tile_elems: int, slab_rows: int, center_ptr,
-                                weights: Sequence[float], n_elems: int, max_norm: float, out_ptr: int, out_code: int,
-                                norms_ptr, ws_ptr: int, ws_bytes: int, stream_ptr: int) -> None:
-    """dla_wsum_bounded_slab_tiled over rows 0..len(weights)-1 (center_ptr None: row 0 is the centre)."""
+                                weights: Sequence[float], *args) -> None:
+    """dla_wsum_bounded_slab_tiled over rows 0..len(weights)-1 (center_ptr None: row 0 is the centre): n_elems,
+    max_norm, out, out_dtype, norms, counters, workspace, bytes, stream."""
     L = lib()
-    L.check(L.so.dla_wsum_bounded_slab_tiled(dtype_code, base_ptr, tile_elems, slab_rows, center_ptr, _dbl_array(weights),
-                                             len(weights), n_elems, max_norm, out_ptr, out_code, norms_ptr, ws_ptr,
-                                             ws_bytes, stream_ptr), "dla_wsum_bounded_slab_tiled")
+    rc = L.so.dla_wsum_bounded_slab_tiled(dtype_code, base_ptr, tile_elems, slab_rows, center_ptr, _dbl_array(weights),
+                                          len(weights), *args)
+    if rc:
+        L.check(rc, "dla_wsum_bounded_slab_tiled")
 
 
 def wsum_slab_ptr(dtype_code: int, base_ptr: int, pitch_elems: int, weights: Sequence[float], n_peers: int,

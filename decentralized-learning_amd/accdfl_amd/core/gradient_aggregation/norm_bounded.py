@@ -49,10 +49,10 @@ def _device_round(models: List[nn.Module], weights, center: nn.Module, max_norm:
     with _norms._place(device, None):
         blocks, out_ptrs = mod.param_blocks(p0)
         address = ctypes.c_void_p * t
-        tables = _norms._Tables(t, device, (ctypes.c_int * t)(*[_wsum.dtype_code(dtype)] * t),
+        tables = _norms._Tables(device.index, dtype == torch.float64, (ctypes.c_int * t)(*[_wsum.dtype_code(dtype)] * t),
                                 _fedavg._flat_plan(dtype, numels)[3], [address.from_buffer(table[:, 0].copy())],
-                                (ctypes.c_void_p * (t * n)).from_buffer(table[:, 1:].copy()), dtype == torch.float64)
-        _norms.wsum_bounded_tables(tables, address.from_buffer(out_ptrs), weights, n, max_norm)
+                                (ctypes.c_void_p * (t * n)).from_buffer(table[:, 1:].copy()))
+        _norms.wsum_bounded_tables(tables, out_ptrs.ctypes.data, weights, n, max_norm)
         # while the round runs: the parameters' Python objects, models[0]'s buffers, the module tree
         mod.param_wrap(blocks, p0, memo)
         _fedavg._seed_buffers(b0, memo)

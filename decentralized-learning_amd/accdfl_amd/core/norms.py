@@ -25,7 +25,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-from typing import Iterable, List, Optional, Sequence, Tuple, Union
+from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import nn
@@ -41,44 +41,30 @@ MAX_PEERS = 2048  # include/dlagg.h dla_peer_workspace
 
 # ------------------------------------------------------------------------------------------- tables of tensors
 class _Tables:
-    """What one call hands to the library: dtype codes and counts of T tensors, the addresses of the first
-    ``lead`` lists, and those of the other lists tensor-major."""
+    """What one call hands to the library, with the attributes of the walk extension's DenseTables: ``n`` tensors on
+    HIP device ``device``, ``wide``: float64 among them, and the addresses of the tables — dtype codes, counts, the
+    i-th of the first lists, the other lists tensor-major.  ``keep``: what owns them."""
 
-    __slots__ = ("n", "device", "codes", "numels", "lead", "rest", "wide")
+    __slots__ = ("n", "device", "wide", "codes", "numels", "leads", "rest", "keep")
 
-    def __init__(self, n, device, codes, numels, lead, rest, wide):
-        self.n = n
+    def __init__(self, device: int, wide: bool, codes, numels, leads, rest):
+        self.n = len(codes)
         self.device = device
-        self.codes = codes
-        self.numels = numels
-        self.lead = lead
-        self.rest = rest
-        self.wide = wide  # float64 among the tensors
+        self.wide = wide
+        self.keep = (codes, numels, leads, rest)
+        self.codes, self.numels = ctypes.addressof(codes), ctypes.addressof(numels)
+        self.leads = [ctypes.addressof(x) for x in leads]
+        self.rest = None if rest is None else ctypes.addressof(rest)
 
-    @property
-    def out_dtype(self) -> torch.dtype:
-        return torch.float64 if self.wide else torch.float32
-
-    @property
-    def out_code(self) -> int:
-        return _lib.DLA_F64 if self.wide else _lib.DLA_F32
+    def lead(self, i: int) -> int:
+        return self.leads[i]
 
 
-def _pack(lists: List[List[torch.Tensor]], lead: int, bump: int = -1) -> Optional[_Tables]:
+def _pack(lists: List[List[torch.Tensor]], lead: int, bump: int = -1):
     """The tables of lists whose tensors the kernels take as they are (walk.cpp dense_lists), else None.
     ``bump``: the list that the call writes (its tensors' version counters move on)."""
     mod = _lib.walk_module()
-    if mod is None:
-        return None
-    r = mod.dense_lists(lists, lead, bump)
-    if r is None:
-        return None
-    device, codes, numels, head, tail, wide = r
-    n = len(lists[0])
-    row = ctypes.c_void_p * n
-    return _Tables(n, torch.device("cuda", device), (ctypes.c_int * n).from_buffer(codes),
-                   (ctypes.c_int64 * n).from_buffer(numels), [row.from_buffer(head, 8 * n * i) for i in range(lead)],
-                   (ctypes.c_void_p * (len(tail) // 8)).from_buffer(tail) if len(tail) else None, wide)
+    return None if mod is None else mod.dense_lists(lists, lead, bump)
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -147,11 +133,11 @@ def _pack_checked(lists: List[List[torch.Tensor]], names: Sequence[str], lead: i
         n, rest = len(lists[0]), lists[lead:]
         row = ctypes.c_void_p * n
         address = lambda t: t.data_ptr() if t.numel() else 0  # noqa: E731
-        tables = _Tables(n, device, (ctypes.c_int * n)(*[_wsum.dtype_code(t.dtype) for t in lists[0]]),
+        tables = _Tables(device.index, any(t.dtype == torch.float64 for t in lists[0]), (ctypes.c_int * n)(*[_wsum.dtype_code(t.dtype) for t in lists[0]]),
                          (ctypes.c_int64 * n)(*[t.numel() for t in lists[0]]),
                          [row(*[address(t) for t in ts]) for ts in lists[:lead]],
                          (ctypes.c_void_p * (n * len(rest)))(*[address(ts[i]) for i in range(n) for ts in rest])
-                         if rest else None, any(t.dtype == torch.float64 for t in lists[0]))
+                         if rest else None)
         if out >= 0:
             torch.autograd.graph.increment_version([t for t in lists[out] if not t.is_inference()])
     return tables, back, lists  # the lists keep the copies alive until the call is enqueued
@@ -197,8 +183,8 @@ def _place(device: torch.device, stream: Optional[torch.cuda.Stream]):
     return _placed(device, stream)
 
 
-def _raw_stream(device: torch.device) -> int:
-    return int(torch.cuda.current_stream(device).cuda_stream)
+def _raw_stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _device_of(tensors: List[torch.Tensor], stream: Optional[torch.cuda.Stream]) -> torch.device:
@@ -208,8 +194,30 @@ def _device_of(tensors: List[torch.Tensor], stream: Optional[torch.cuda.Stream])
     return stream.device if stream is not None else _wsum.require_device(None)
 
 
-def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+def _workspace(nbytes: int, device: int) -> torch.Tensor:
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _result_type(tables):
+    """(torch dtype, DLA_* code) of a call's norms."""
+    return (torch.float64, _lib.DLA_F64) if tables.wide else (torch.float32, _lib.DLA_F32)
+
+
+# Counters of the library's last-workgroup joins (include/dlagg.h): zero before and after every call, so the calls of
+# one stream share one set — (device, stream handle) -> tensor.  A captured call takes none (a replay may run on
+# another stream): it joins in a launch of its own.  Nor does hipStreamPerThread, one handle for many streams.
+_counters: Dict[Tuple[int, int], torch.Tensor] = {}
+_STREAM_PER_THREAD = 2
+
+
+def _counter(device: int, raw_stream: int) -> Optional[int]:
+    if raw_stream == _STREAM_PER_THREAD or torch.cuda.is_current_stream_capturing():
+        return None
+    t = _counters.get((device, raw_stream))
+    if t is None:
+        t = _counters.setdefault((device, raw_stream), torch.zeros(_lib.COUNTER_BYTES // 4, dtype=torch.int32,
+                                                                   device=device))
+    return t.data_ptr()
 
 
 def _refuse_nonfinite(norm: torch.Tensor, norm_type: float) -> None:
@@ -239,11 +247,13 @@ def global_norm(tensors: Tensors, norm_type: float = 2.0, error_if_nonfinite: bo
         tables, keep = _pack([tensors], 1), None
         if tables is None:
             tables, _, keep = _pack_checked([tensors], ["tensors"], 1)
-        out = torch.empty((), dtype=tables.out_dtype, device=tables.device)
+        dtype, out_code = _result_type(tables)
+        out = torch.empty((), dtype=dtype, device=tables.device)
         nbytes = _lib.norm_workspace(tables.n)
         ws = _workspace(nbytes, tables.device)
-        _lib.norm_ptrs(tables.n, tables.codes, tables.lead[0], tables.numels, code, tables.out_code, out.data_ptr(),
-                       ws.data_ptr(), nbytes, _raw_stream(tables.device))
+        raw = _raw_stream(tables.device)
+        _lib.norm_ptrs(tables.n, tables.codes, tables.lead(0), tables.numels, code, out_code, out.data_ptr(),
+                       _counter(tables.device, raw), ws.data_ptr(), nbytes, raw)
         del keep
         if error_if_nonfinite:
             _refuse_nonfinite(out, norm_type)
@@ -275,16 +285,18 @@ def clip_global_norm(tensors: Tensors, max_norm: float, norm_type: float = 2.0, 
         tables, back, keep = _pack([tensors, outs], 2, bump=1), (), None
         if tables is None:
             tables, back, keep = _pack_checked([tensors, outs], ["tensors", "outs"], 2, out=1)
-        norm = torch.empty((), dtype=tables.out_dtype, device=tables.device)
+        dtype, out_code = _result_type(tables)
+        norm = torch.empty((), dtype=dtype, device=tables.device)
         nbytes = _lib.norm_workspace(tables.n)
         ws = _workspace(nbytes, tables.device)
         raw = _raw_stream(tables.device)
-        _lib.norm_ptrs(tables.n, tables.codes, tables.lead[0], tables.numels, code, tables.out_code,
-                       norm.data_ptr() if error_if_nonfinite else None, ws.data_ptr(), nbytes, raw)
+        counter = _counter(tables.device, raw)
         if error_if_nonfinite:
+            _lib.norm_ptrs(tables.n, tables.codes, tables.lead(0), tables.numels, code, out_code, norm.data_ptr(),
+                           counter, ws.data_ptr(), nbytes, raw)
             _refuse_nonfinite(norm, norm_type)
-        _lib.norm_scale_ptrs(tables.n, tables.codes, tables.lead[0], tables.lead[1], tables.numels, code, bound, CLIP_EPS,
-                             tables.out_code, norm.data_ptr(), ws.data_ptr(), nbytes, raw)
+        _lib.norm_clip_ptrs(tables.n, tables.codes, tables.lead(0), tables.lead(1), tables.numels, code, bound, CLIP_EPS,
+                            out_code, norm.data_ptr(), counter, ws.data_ptr(), nbytes, raw)
         for t, copy in back:
             t.copy_(copy)
         del keep
@@ -321,6 +333,25 @@ def _check_peers(n: int) -> None:
         raise ValueError("%d peers: at most %d in one call" % (n, MAX_PEERS))
 
 
+@contextlib.contextmanager
+def _table_host(n_tensors: int, n: int, device: int):
+    """(address, bytes) of page-locked memory for a round's table, or (None, 0): the table is small enough to go with
+    the launches, the call is being captured (its launches then carry the table by value), or every slot of the
+    device's ring is in use."""
+    nbytes = _lib.peer_table(n_tensors, n)
+    slot = None
+    if nbytes and not torch.cuda.is_current_stream_capturing():
+        ring = _wsum.table_ring(torch.device("cuda", device))
+        slot = ring.take(nbytes, wait=False)
+    if slot is None:
+        yield None, 0
+        return
+    try:
+        yield slot[1].data_ptr(), nbytes
+    finally:
+        ring.done(slot[0], torch.cuda.current_stream(device), fence=True)
+
+
 def update_norms(models: Sequence[Tensors], center: Tensors, stream: Optional[torch.cuda.Stream] = None,
                  squared: bool = False) -> torch.Tensor:
     """``|| model_k - center ||_2`` over all tensors of each model (lists of tensors, modules' parameters, or flat
@@ -334,26 +365,32 @@ def update_norms(models: Sequence[Tensors], center: Tensors, stream: Optional[to
         if not lists[0] and not any(lists):
             return torch.zeros(n, dtype=torch.float64 if squared else torch.float32, device=device)
         tables, _, keep = _pack_round(lists, lambda: ["center"] + ["model %d" % k for k in range(n)], 1)
-        out = torch.empty(n, dtype=torch.float64 if squared else tables.out_dtype, device=tables.device)
+        dtype, out_code = _result_type(tables)
+        out = torch.empty(n, dtype=torch.float64 if squared else dtype, device=tables.device)
         nbytes = _lib.peer_workspace(tables.n, n)
         ws = _workspace(nbytes, tables.device)
-        _lib.peer_norms_ptrs(tables.n, tables.codes, tables.rest, tables.lead[0], tables.numels, n,
-                             out.data_ptr() if squared else None, tables.out_code, None if squared else out.data_ptr(),
-                             ws.data_ptr(), nbytes, _raw_stream(tables.device))
+        raw = _raw_stream(tables.device)
+        with _table_host(tables.n, n, tables.device) as (host, host_bytes):
+            _lib.peer_norms_ptrs(tables.n, tables.codes, tables.rest, tables.lead(0), tables.numels, n,
+                                 out.data_ptr() if squared else None, out_code, None if squared else out.data_ptr(),
+                                 _counter(tables.device, raw), host, host_bytes, ws.data_ptr(), nbytes, raw)
         del keep
         return out
 
 
-def wsum_bounded_tables(tables: _Tables, outs, weights: Sequence[float], n: int, max_norm: float,
+def wsum_bounded_tables(tables, outs: int, weights: Sequence[float], n: int, max_norm: float,
                         sq_norms: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """dla_wsum_bounded on packed tables (``tables.lead[0]`` the centre, ``tables.rest`` the peers, ``outs`` a
-    ctypes array of addresses) on the current stream; returns the update norms [n]."""
-    norms = torch.empty(n, dtype=tables.out_dtype, device=tables.device)
+    """dla_wsum_bounded on packed tables (``lead(0)`` the centre, ``rest`` the peers, ``outs`` the address of the
+    outputs' table) on the current stream; returns the update norms [n]."""
+    dtype, out_code = _result_type(tables)
+    norms = torch.empty(n, dtype=dtype, device=tables.device)
     nbytes = _lib.peer_workspace(tables.n, n)
     ws = _workspace(nbytes, tables.device)
-    _lib.wsum_bounded_ptrs(tables.n, tables.codes, tables.rest, tables.lead[0], outs, tables.numels, weights, n, max_norm,
-                           None if sq_norms is None else sq_norms.data_ptr(), tables.out_code, norms.data_ptr(),
-                           ws.data_ptr(), nbytes, _raw_stream(tables.device))
+    raw = _raw_stream(tables.device)
+    with _table_host(tables.n, n, tables.device) as (host, host_bytes):
+        _lib.wsum_bounded_ptrs(tables.n, tables.codes, tables.rest, tables.lead(0), outs, tables.numels, weights, n,
+                               max_norm, None if sq_norms is None else sq_norms.data_ptr(), out_code, norms.data_ptr(),
+                               _counter(tables.device, raw), host, host_bytes, ws.data_ptr(), nbytes, raw)
     return norms
 
 
@@ -382,9 +419,9 @@ def wsum_bounded_multi(peer_params: Sequence[Tensors], weights: Sequence[float],
             return torch.zeros(n, dtype=torch.float32, device=device) if sq_norms is None else sq_norms.sqrt().float()
         tables, back, keep = _pack_round(lists, lambda: ["center", "outs"] + ["peer %d" % k for k in range(n)], 2, out=1)
         if sq_norms is not None and (sq_norms.dtype != torch.float64 or sq_norms.numel() != n
-                                     or sq_norms.device != tables.device or not sq_norms.is_contiguous()):
-            raise ValueError("sq_norms must be %d contiguous float64 values on %s" % (n, tables.device))
-        norms = wsum_bounded_tables(tables, tables.lead[1], weights, n, bound, sq_norms)
+                                     or sq_norms.device != device or not sq_norms.is_contiguous()):
+            raise ValueError("sq_norms must be %d contiguous float64 values on %s" % (n, device))
+        norms = wsum_bounded_tables(tables, tables.lead(1), weights, n, bound, sq_norms)
         for t, copy in back:
             t.copy_(copy)
         del keep

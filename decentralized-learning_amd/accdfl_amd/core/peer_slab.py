@@ -384,11 +384,12 @@ class PeerSlab:
             wide = self.dtype == torch.float64
             norms = torch.empty(n, dtype=torch.float64 if wide else torch.float32, device=self.device)
             nbytes = _lib.peer_workspace(1, n)
-            ws = _norms._workspace(nbytes, self.device)
+            ws = _norms._workspace(nbytes, self.device.index)
+            raw = int(cur.cuda_stream)
             _lib.wsum_bounded_slab_tiled_ptr(self.code, self.buf.data_ptr(), self.tile, self.capacity,
                                              None if row is None else row.data_ptr(), weights, self.total, bound,
                                              out.data_ptr(), _lib.DLA_F64 if wide else _lib.DLA_F32, norms.data_ptr(),
-                                             ws.data_ptr(), nbytes, int(cur.cuda_stream))
+                                             _norms._counter(self.device.index, raw), ws.data_ptr(), nbytes, raw)
         return out, norms
 
     def reduce_bounded_into(self, params: Sequence[torch.Tensor], max_norm: float,

@@ -205,14 +205,17 @@ class _TableRing:
             self.fence[idx] = ev
         self.pending = []
 
-    def take(self, nbytes: int):
-        """(slot index, host buffer, device buffer); the caller passes the index to done()."""
+    def take(self, nbytes: int, wait: bool = True):
+        """(slot index, host buffer, device buffer); the caller passes the index to done().  ``wait=False``: None
+        instead of an error when every slot is in use by another thread's call."""
         with self.lock:
             for _ in range(self.SLOTS):
                 self.i = (self.i + 1) % self.SLOTS
                 if not self.busy[self.i]:
                     break
             else:
+                if not wait:
+                    return None
                 raise RuntimeError("wsum_multi_table: more than %d concurrent calls on %s" % (self.SLOTS, self.device))
             idx = self.i
             self.busy[idx] = True
@@ -229,18 +232,29 @@ class _TableRing:
             self.slots[idx] = slot
         return idx, slot[0], slot[1]
 
-    def done(self, idx: int, stream: torch.cuda.Stream):
+    def done(self, idx: int, stream: torch.cuda.Stream, fence: bool = False):
+        """``fence``: record the slot's event now, so that none is left to be recorded on ``stream`` later (a stream
+        that may be captured by then)."""
         with self.lock:
             self.busy[idx] = False
             if self.pending and self.pending[-1][1].cuda_stream != stream.cuda_stream:
                 self._fence_locked()
             self.pending.append((idx, stream))
-            if len(self.pending) >= self.FENCE_EVERY:
+            if fence or len(self.pending) >= self.FENCE_EVERY:
                 self._fence_locked()
 
 
 _rings = {}
 _rings_lock = threading.Lock()
+
+
+def table_ring(device: torch.device) -> _TableRing:
+    """The device's ring of table buffers."""
+    with _rings_lock:
+        ring = _rings.get(device)
+        if ring is None:
+            ring = _rings[device] = _TableRing(device)
+    return ring
 
 
 _table_bytes = {}  # (n_tensors, n_peers) -> dla_wsum_multi_table_bytes
@@ -261,10 +275,7 @@ def wsum_multi_ptrs(dtype: torch.dtype, ptrs, out_ptrs, numels, weights: Sequenc
         n > 8 and (n + 1) * (sum(numels) if total_elems is None else total_elems) * _ESIZE[dtype]
         >= MULTI_TABLE_MIN_BYTES)
     if table and (dtype != torch.float64 or acc_in):  # fp64 folds per tensor inside the table call
-        with _rings_lock:
-            ring = _rings.get(device)
-            if ring is None:
-                ring = _rings[device] = _TableRing(device)
+        ring = table_ring(device)
         key = (len(out_ptrs), n)
         nbytes = _table_bytes.get(key)
         if nbytes is None:

@@ -15,10 +15,10 @@
 // underflows.  A result is rounded to its storage type once (16-bit types through f32: the second
 // rounding moves a result by less than 2^-24 of itself before the last one).
 //
-// Work is cut into units of 4 KiB (16 bytes per lane of a 256-thread workgroup) or 16 KiB of one tensor;
-// a unit never spans tensors.  Workgroup b of P takes units [b U / P, (b + 1) U / P): one partial result
-// per workgroup whatever the size, added up in a fixed order by the kernel that needs the sum, so the
-// results do not depend on which workgroup ended first.  Loads need element alignment only (gfx950
+// Work is cut into units of 1 to 32 KiB of one tensor; a unit never spans tensors.  Workgroup b of P takes units b, b + P, b + 2 P, ...: the chip walks every
+// stream as one front (few DRAM rows and pages at a time), and there is one partial result per workgroup
+// whatever the size, added up in a fixed order by the kernel that needs the sum, so the results do not
+// depend on which workgroup ended first.  Loads need element alignment only (gfx950
 // takes 16-byte loads from any address), so tensors that start anywhere take the same path.
 #include <hip/hip_runtime.h>
 
@@ -28,6 +28,7 @@
 #include <cstring>
 #include <exception>
 #include <string>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -86,14 +87,16 @@ template <> struct Elem<DLA_F64> {
 template <> struct Elem<DLA_BF16> {
   using bits = uint16_t;
   static constexpr int E = 8;
-  static __device__ inline void widen(u32x4 r, double (&v)[E]) {
+  template <class R>
+  static __device__ inline void widen(u32x4 r, R (&v)[E]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[2 * i] = static_cast<double>(__uint_as_float(r[i] << 16));
-      v[2 * i + 1] = static_cast<double>(__uint_as_float(r[i] & 0xffff0000u));
+      v[2 * i] = static_cast<R>(__uint_as_float(r[i] << 16));
+      v[2 * i + 1] = static_cast<R>(__uint_as_float(r[i] & 0xffff0000u));
     }
   }
-  static __device__ inline u32x4 narrow(const double (&v)[E]) {
+  template <class R>
+  static __device__ inline u32x4 narrow(const R (&v)[E]) {
     typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
     typedef float f2 __attribute__((ext_vector_type(2)));
     u32x4 r;
@@ -112,17 +115,19 @@ template <> struct Elem<DLA_F16> {
   using bits = uint16_t;
   static constexpr int E = 8;
   typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-  static __device__ inline void widen(u32x4 r, double (&v)[E]) {
+  template <class R>
+  static __device__ inline void widen(u32x4 r, R (&v)[E]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       h2 h;
       const uint32_t w = r[i];
       __builtin_memcpy(&h, &w, 4);
-      v[2 * i] = static_cast<double>(static_cast<float>(h[0]));
-      v[2 * i + 1] = static_cast<double>(static_cast<float>(h[1]));
+      v[2 * i] = static_cast<R>(static_cast<float>(h[0]));
+      v[2 * i + 1] = static_cast<R>(static_cast<float>(h[1]));
     }
   }
-  static __device__ inline u32x4 narrow(const double (&v)[E]) {
+  template <class R>
+  static __device__ inline u32x4 narrow(const R (&v)[E]) {
     u32x4 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -135,6 +140,28 @@ template <> struct Elem<DLA_F16> {
     return r;
   }
 };
+
+// The average's arithmetic: out = c + sum_k a_k (x_k - c).  In 64 bits for F32 and F64.  16-bit types, whose
+// result keeps 8 or 11 bits, take 32: twice the elements per register and a quarter of the conversions.  There
+// the difference is taken of halves, one fma (x / 2 - c / 2) with the 2 in the share, so that two values at
+// opposite ends of bf16's range do not overflow it.
+template <int DT>
+struct Average {
+  using real = double;
+  static __device__ inline double share(double a) { return a; }
+  static __device__ inline double center(double c) { return c; }
+  static __device__ inline double update(double x, double c) { return x - c; }
+  static __device__ inline double fold(double a, double d, double acc) { return __builtin_fma(a, d, acc); }
+};
+struct Average16 {
+  using real = float;
+  static __device__ inline float share(double a) { return static_cast<float>(2.0 * a); }
+  static __device__ inline float center(float c) { return -0.5f * c; }
+  static __device__ inline float update(float x, float c) { return __builtin_fmaf(0.5f, x, c); }
+  static __device__ inline float fold(float a, float d, float acc) { return __builtin_fmaf(a, d, acc); }
+};
+template <> struct Average<DLA_BF16> : Average16 {};
+template <> struct Average<DLA_F16> : Average16 {};
 
 // Elements [j, j + n) of a tensor, n <= E: 16 bytes at once when n == E, else one by one with zeros behind.
 template <int DT>
@@ -150,10 +177,13 @@ __device__ inline u32x4 load_part(const void* base, int64_t j, int n) {
   __builtin_memcpy(&r, v, 16);
   return r;
 }
-template <int DT>
+// NT: non-temporal, for data that no cache will hold until it is read again.
+template <int DT, bool NT = true>
 __device__ inline u32x4 load_full(const void* base, int64_t j) {
   using B = typename Elem<DT>::bits;
-  return *(const u32x4_any __attribute__((address_space(1)))*)(global_ptr<B>(base) + j);
+  const auto* p = (const u32x4_any __attribute__((address_space(1)))*)(global_ptr<B>(base) + j);
+  if (NT) return __builtin_nontemporal_load(p);
+  return *p;
 }
 template <int DT>
 __device__ inline void store_part(void* base, int64_t j, int n, u32x4 r) {
@@ -161,7 +191,7 @@ __device__ inline void store_part(void* base, int64_t j, int n, u32x4 r) {
   constexpr int E = Elem<DT>::E;
   auto* p = global_ptr<B>(base) + j;
   if (n >= E) {
-    *(u32x4_any __attribute__((address_space(1)))*)p = r;
+    __builtin_nontemporal_store(r, (u32x4_any __attribute__((address_space(1)))*)p);
     return;
   }
   B v[E];
@@ -202,10 +232,31 @@ __device__ inline double block_join(double v, double* lds) {
   __syncthreads();
   return s;
 }
+// Partial results that another workgroup of the same kernel reads go past the L2 of the XCD that wrote them, both
+// ways (agent-scope atomics): no workgroup has to write back or invalidate an L2, which a fence of that scope does
+// and which cost 40 us over 1 024 workgroups.
+__device__ inline void publish(double* p, double v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline double published(const double* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Partials i, i + step, ... of n, in order; 8 loads in flight (each of them is a trip to memory).
+template <int NORM>
+__device__ inline double join_strided(const double* p, int n, int i, int step) {
+  double v = 0;
+  for (; i < n; i += 8 * step) {
+    double r[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) r[q] = i + q * step < n ? published(p + i + q * step) : 0.0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v = norm_join<NORM>(v, r[q]);
+  }
+  return v;
+}
 template <int NORM>
 __device__ inline double join_partials(const double* partials, int n, double* lds) {
-  double v = 0;
-  for (int i = threadIdx.x; i < n; i += kThreads) v = norm_join<NORM>(v, global_ptr<double>(partials)[i]);
+  const double v = join_strided<NORM>(partials, n, static_cast<int>(threadIdx.x), kThreads);
   const double s = block_join<NORM>(v, lds);
   return NORM == DLA_NORM_L2 ? __builtin_sqrt(s) : s;
 }
@@ -220,8 +271,8 @@ __device__ inline void put_norm(void* out, int i, int out_dt, double v) {
 // -------------------------------------------------- one list of tensors: norm, and scaling by it
 // A launch's tensors travel in the kernel arguments (nothing to copy, nothing a captured graph could find
 // changed at replay): as many as fit 4 KB.
-constexpr int kVec = 4;                             // 16-byte loads in flight per lane
-constexpr int kUnitBytes = kThreads * 16 * kVec;    // 16 KiB of one tensor
+constexpr int kNormVec = 8, kScaleVec = 4;          // 16-byte loads in flight per lane: units of 32 and 16 KiB
+constexpr int unit_bytes(int vec) { return kThreads * 16 * vec; }
 constexpr int kNormTensors = 190, kScaleTensors = 140;
 constexpr int kMaxPartials = 1024;                  // workgroups of a list's norm: 4 per CU
 
@@ -245,14 +296,14 @@ __device__ inline int find_tensor(const uint32_t* unit0, int count, uint32_t u) 
   return __builtin_amdgcn_readfirstlane(n) - 1;
 }
 
-template <int NORM, int DT>
-__device__ inline void norm_unit(const void* p, int64_t n, int64_t unit, double (&acc)[kVec]) {
-  constexpr int E = Elem<DT>::E;
+template <int NORM, int DT, bool NT>
+__device__ inline void norm_unit(const void* p, int64_t n, int64_t unit, double (&acc)[kNormVec]) {
+  constexpr int E = Elem<DT>::E, kVec = kNormVec;
   const int64_t j0 = unit * (kThreads * kVec * E) + static_cast<int>(threadIdx.x) * E;
   u32x4 r[kVec];
   if ((unit + 1) * (kThreads * kVec * E) <= n) {
 #pragma unroll
-    for (int v = 0; v < kVec; ++v) r[v] = load_full<DT>(p, j0 + v * (kThreads * E));
+    for (int v = 0; v < kVec; ++v) r[v] = load_full<DT, NT>(p, j0 + v * (kThreads * E));
   } else {
 #pragma unroll
     for (int v = 0; v < kVec; ++v) {
@@ -269,36 +320,71 @@ __device__ inline void norm_unit(const void* p, int64_t n, int64_t unit, double 
   }
 }
 
-// Workgroup b's part of the norm of a list: partials[b].
-template <int NORM>
+// True in every thread of the last of a kernel's workgroups to get here, which then sees what the others' first
+// threads published before they did: their stores have completed (vmcnt counts them) when the counter is raised.
+// The counters are zero when the kernel starts and zero again when it has ended (they wrap).  Workgroups of one
+// row (blockIdx.y) count together: many of them in two steps, 32 counters and then one, because a thousand
+// increments of one address take 15 us.
+constexpr int kCounterSlots = DLA_COUNTER_BYTES / 128, kSlot = 32;  // one counter per 128-byte line
+constexpr uint32_t kFan = 32, kFanFrom = 64;
+__device__ inline bool last_to_arrive(uint32_t* counters) {
+  __shared__ bool last;
+  if (threadIdx.x == 0) {
+    const uint32_t n = gridDim.x, b = blockIdx.x;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (n >= kFanFrom && gridDim.y * (kFan + 1) <= kCounterSlots) {
+      uint32_t* mine = counters + blockIdx.y * ((kFan + 1) * kSlot);
+      const uint32_t fan = b % kFan, of = (n - fan + kFan - 1) / kFan;
+      last = atomicInc(mine + (1 + fan) * kSlot, of - 1) == of - 1 && atomicInc(mine, kFan - 1) == kFan - 1;
+    } else {
+      last = atomicInc(counters + blockIdx.y * kSlot, n - 1) == n - 1;
+    }
+    asm volatile("" ::: "memory");
+  }
+  __syncthreads();
+  return last;
+}
+
+// Workgroup b's part of the norm of a list: partials[b].  With a counter, the last workgroup joins the `joined`
+// partials (this launch's and those of the launches before it) into *norm and *out.
+template <int NORM, bool NT>
 __global__ __launch_bounds__(kThreads) void norm_kernel(const TensorList<kNormTensors> tab, int count, uint32_t units,
-                                                        double* partials) {
+                                                        double* to, uint32_t* counter, const double* partials,
+                                                        int joined, double* norm, int out_dt, void* out) {
   __shared__ double lds[kWaves];
   const uint32_t b = blockIdx.x, nb = gridDim.x;
-  uint32_t u = static_cast<uint32_t>(static_cast<uint64_t>(units) * b / nb);
-  const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(units) * (b + 1) / nb);
-  int t = find_tensor(tab.unit0, count, u);
-  double acc[kVec] = {};
-  while (u < end) {
-    const uint32_t first = tab.unit0[t];
-    uint32_t stop = t + 1 < count ? tab.unit0[t + 1] : units;
-    if (stop > end) stop = end;
-    const void* p = tab.p[t];
-    const uint64_t nd = tab.n_dt[t];
+  uint32_t first = 0, stop = 0;
+  const void* p = nullptr;
+  uint64_t nd = 0;
+  double acc[kNormVec] = {};
+  for (uint64_t at = b; at < units; at += nb) {
+    const uint32_t u = static_cast<uint32_t>(at);
+    if (u >= stop) {
+      const int t = find_tensor(tab.unit0, count, u);
+      first = tab.unit0[t];
+      stop = t + 1 < count ? tab.unit0[t + 1] : units;
+      p = tab.p[t];
+      nd = tab.n_dt[t];
+    }
     const int64_t n = static_cast<int64_t>(nd >> 2);
     switch (nd & 3) {
-      case DLA_F32: for (; u < stop; ++u) norm_unit<NORM, DLA_F32>(p, n, u - first, acc); break;
-      case DLA_BF16: for (; u < stop; ++u) norm_unit<NORM, DLA_BF16>(p, n, u - first, acc); break;
-      case DLA_F16: for (; u < stop; ++u) norm_unit<NORM, DLA_F16>(p, n, u - first, acc); break;
-      default: for (; u < stop; ++u) norm_unit<NORM, DLA_F64>(p, n, u - first, acc); break;
+      case DLA_F32: norm_unit<NORM, DLA_F32, NT>(p, n, u - first, acc); break;
+      case DLA_BF16: norm_unit<NORM, DLA_BF16, NT>(p, n, u - first, acc); break;
+      case DLA_F16: norm_unit<NORM, DLA_F16, NT>(p, n, u - first, acc); break;
+      default: norm_unit<NORM, DLA_F64, NT>(p, n, u - first, acc); break;
     }
-    ++t;
   }
   double v = acc[0];
 #pragma unroll
-  for (int i = 1; i < kVec; ++i) v = norm_join<NORM>(v, acc[i]);
+  for (int i = 1; i < kNormVec; ++i) v = norm_join<NORM>(v, acc[i]);
   v = block_join<NORM>(v, lds);
-  if (threadIdx.x == 0) global_ptr<double>(partials)[b] = v;
+  if (threadIdx.x == 0) publish(to + b, v);
+  if (!counter || !last_to_arrive(counter)) return;
+  v = join_partials<NORM>(partials, joined, lds);
+  if (threadIdx.x == 0) {
+    *global_ptr<double>(norm) = v;
+    if (out) put_norm(out, 0, out_dt, v);
+  }
 }
 
 template <int NORM>
@@ -308,9 +394,9 @@ __global__ __launch_bounds__(kThreads) void norm_join_kernel(const double* parti
   if (threadIdx.x == 0) put_norm(out, 0, out_dt, v);
 }
 
-template <int DT>
+template <int DT, bool NT>
 __device__ inline void scale_unit(const void* p, void* out, int64_t n, int64_t unit, double ratio) {
-  constexpr int E = Elem<DT>::E;
+  constexpr int E = Elem<DT>::E, kVec = kScaleVec;
   const int64_t j0 = unit * (kThreads * kVec * E) + static_cast<int>(threadIdx.x) * E;
   const bool full = (unit + 1) * (kThreads * kVec * E) <= n;
   u32x4 r[kVec];
@@ -319,7 +405,7 @@ __device__ inline void scale_unit(const void* p, void* out, int64_t n, int64_t u
   for (int v = 0; v < kVec; ++v) {
     const int64_t j = j0 + v * (kThreads * E);
     part[v] = full ? E : clamp_part(n - j, E);
-    r[v] = full ? load_full<DT>(p, j) : load_part<DT>(p, j, part[v]);
+    r[v] = full ? load_full<DT, NT>(p, j) : load_part<DT>(p, j, part[v]);
   }
 #pragma unroll
   for (int v = 0; v < kVec; ++v) {
@@ -331,58 +417,62 @@ __device__ inline void scale_unit(const void* p, void* out, int64_t n, int64_t u
   }
 }
 
-// y = round(x * min(1, M / (n + eps))).  Every workgroup joins the partials itself (8 KB that all of them
-// read: less than a launch between the two kernels costs) and then walks its units backwards: what the
-// norm read last is what the caches still hold.
-template <int NORM>
+// y = round(x * min(1, M / (n + eps))).  One unit per workgroup, dealt from the last to the first: what the norm
+// read last is what the caches still hold, and the front stays narrow (0.87 G bf16: 561 us, where 2 048 workgroups
+// walking their units took 630).
+template <bool NT>
 __global__ __launch_bounds__(kThreads) void norm_scale_kernel(const TensorsInOut<kScaleTensors> tab, int count,
-                                                              uint32_t units, const double* partials, int n_partials,
-                                                              double max_norm, double eps, int in_place, int out_dt,
-                                                              void* norm_out) {
-  __shared__ double lds[kWaves];
-  const double norm = join_partials<NORM>(partials, n_partials, lds);
+                                                              uint32_t units, const double* joined, double max_norm,
+                                                              double eps, int in_place, int out_dt, void* norm_out) {
+  const double norm = *const_ptr<double>(joined);
   const uint32_t b = blockIdx.x, nb = gridDim.x;
   if (b == 0 && threadIdx.x == 0 && norm_out) put_norm(norm_out, 0, out_dt, norm);
   const double q = max_norm / (norm + eps);
   const double ratio = q > 1.0 ? 1.0 : q;  // NaN stays NaN
   if (in_place && ratio == 1.0) return;    // x * 1 = x: nothing to write
-  const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(units) * b / nb);
-  uint32_t u = static_cast<uint32_t>(static_cast<uint64_t>(units) * (b + 1) / nb);
-  if (u == begin) return;
-  int t = find_tensor(tab.in.unit0, count, u - 1);
-  while (u > begin) {
-    const uint32_t first = tab.in.unit0[t];
-    const uint32_t stop = first > begin ? first : begin;
-    const void* p = tab.in.p[t];
-    void* out = tab.out[t];
-    const uint64_t nd = tab.in.n_dt[t];
+  uint32_t first = 0xffffffffu;
+  const void* p = nullptr;
+  void* out = nullptr;
+  uint64_t nd = 0;
+  for (int64_t at = static_cast<int64_t>(units) - 1 - b; at >= 0; at -= nb) {
+    const uint32_t u = static_cast<uint32_t>(at);
+    if (u < first) {
+      const int t = find_tensor(tab.in.unit0, count, u);
+      first = tab.in.unit0[t];
+      p = tab.in.p[t];
+      out = tab.out[t];
+      nd = tab.in.n_dt[t];
+    }
     const int64_t n = static_cast<int64_t>(nd >> 2);
     switch (nd & 3) {
-      case DLA_F32: for (; u > stop; --u) scale_unit<DLA_F32>(p, out, n, u - 1 - first, ratio); break;
-      case DLA_BF16: for (; u > stop; --u) scale_unit<DLA_BF16>(p, out, n, u - 1 - first, ratio); break;
-      case DLA_F16: for (; u > stop; --u) scale_unit<DLA_F16>(p, out, n, u - 1 - first, ratio); break;
-      default: for (; u > stop; --u) scale_unit<DLA_F64>(p, out, n, u - 1 - first, ratio); break;
+      case DLA_F32: scale_unit<DLA_F32, NT>(p, out, n, u - first, ratio); break;
+      case DLA_BF16: scale_unit<DLA_BF16, NT>(p, out, n, u - first, ratio); break;
+      case DLA_F16: scale_unit<DLA_F16, NT>(p, out, n, u - first, ratio); break;
+      default: scale_unit<DLA_F64, NT>(p, out, n, u - first, ratio); break;
     }
-    --t;
   }
 }
 
 // ------------------------------------------------------------- peers around a centre
-// The round's table in device memory: a record per tensor, then the peers' pointers (tensor-major), then the
-// weights.  It goes there by value, as arguments of put_kernel, so a captured graph holds its own copy.
+// The round's table: a record per tensor, then the peers' pointers (tensor-major), then the weights.  Up to
+// kPutWords words travel in the kernels' own arguments (14 tensors of 2 peers take 100, one tensor of 128 peers
+// 261); a larger table goes to the workspace first — by a copy kernel that reads the caller's page-locked memory, or
+// by value as arguments of put_kernel, as many launches as it takes, which a captured graph keeps.
 struct Seg {
-  int64_t unit0;  // first unit (4 KiB of one tensor of one peer)
-  int64_t n;
+  int64_t norm_unit0, mean_unit0;  // first unit of the tensor in each of the two kernels' counts
+  uint64_t n_dt;                   // elements * 4 + dtype
   const void* center;
   void* out;
-  int64_t dt;
 };
 struct Layout {      // where element j of a peer (and of the centre) lies, in elements from its pointer:
   int shift;         //   (j >> shift) * stride + (j & (2^shift - 1)) in a tile-interleaved slab
   int64_t stride;
   int64_t center_stride;
 };
-constexpr int kPeerUnit = kThreads * 16;
+constexpr int kPeerVec = 4;                             // 16-byte loads of one peer in a row per lane
+constexpr int kNormUnit = kThreads * 16;                // bytes of one tensor of one peer, times 1 or kPeerVec
+constexpr int kMeanThreads = 64, kMeanSteps = 1;
+constexpr int kMeanUnit = kMeanThreads * 16 * kMeanSteps;
 constexpr int kPutWords = 480;
 struct PutWords {
   uint64_t w[kPutWords];
@@ -391,6 +481,29 @@ __global__ __launch_bounds__(512) void put_kernel(const PutWords words, uint64_t
   const int i = static_cast<int>(threadIdx.x);
   if (i < n) global_ptr<uint64_t>(dst)[i] = words.w[i];
 }
+__global__ __launch_bounds__(kThreads) void fetch_kernel(const uint64_t* src, uint64_t* dst, int64_t n) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (i < n) global_ptr<uint64_t>(dst)[i] = global_ptr<uint64_t>(src)[i];
+}
+
+// Where a kernel finds its table: in the workspace, or in its own first argument (the kernel argument segment is
+// memory like any other).
+struct Table {
+  const uint64_t* at;  // null: in the arguments
+  int count, n_peers;
+};
+struct TableParts {
+  const Seg* segs;
+  const uint64_t* ptrs;
+  const double* weights;
+};
+__device__ inline TableParts parts_of(const Table& tab) {
+  const uint64_t args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  const uint64_t at = tab.at ? reinterpret_cast<uint64_t>(tab.at) : args;
+  const uint64_t ptrs = at + static_cast<uint64_t>(tab.count) * sizeof(Seg);
+  return {reinterpret_cast<const Seg*>(at), reinterpret_cast<const uint64_t*>(ptrs),
+          reinterpret_cast<const double*>(ptrs + static_cast<uint64_t>(tab.count) * tab.n_peers * 8)};
+}
 
 template <bool TILED>
 __device__ inline int64_t place(const Layout& l, int64_t stride, int64_t j) {
@@ -398,215 +511,230 @@ __device__ inline int64_t place(const Layout& l, int64_t stride, int64_t j) {
 }
 
 // The tensor that unit u lies in: a 64-way search by the wave's lanes over the records' first units.
+template <int64_t Seg::*UNIT0>
 __device__ inline int find_seg(const Seg* segs, int count, int64_t u) {
   const int lane = static_cast<int>(threadIdx.x & 63);
   int lo = 0, hi = count;
   while (hi - lo > 1) {
     const int step = (hi - lo + 63) / 64;
     const int i = lo + lane * step;
-    const int below = __popcll(__ballot(i < hi && global_ptr<Seg>(segs)[i < hi ? i : lo].unit0 <= u));
+    const int below = __popcll(__ballot(i < hi && (global_ptr<Seg>(segs) + (i < hi ? i : lo))->*UNIT0 <= u));
     lo = __builtin_amdgcn_readfirstlane(lo + (below - 1) * step);
     hi = lo + step < hi ? lo + step : hi;
   }
   return lo;
 }
 
-template <int DT, int G, bool TILED>
+template <int DT, int G, int V, bool TILED>
 __device__ inline void peer_norm_unit(const Layout& l, const void* center, const void* const (&p)[G], int64_t n,
                                       int64_t unit, double (&acc)[G]) {
   constexpr int E = Elem<DT>::E;
-  const int64_t j = unit * (kThreads * E) + static_cast<int>(threadIdx.x) * E;
-  const int64_t at = place<TILED>(l, l.stride, j), at_c = place<TILED>(l, l.center_stride, j);
-  u32x4 rc, r[G];
-  if ((unit + 1) * (kThreads * E) <= n) {
-    rc = load_full<DT>(center, at_c);
+  const int64_t j0 = unit * (kThreads * V * E) + static_cast<int>(threadIdx.x) * E;
+  u32x4 rc[V], r[G][V];
+  if ((unit + 1) * (kThreads * V * E) <= n) {
 #pragma unroll
-    for (int g = 0; g < G; ++g) r[g] = load_full<DT>(p[g], at);
+    for (int v = 0; v < V; ++v) rc[v] = load_full<DT>(center, place<TILED>(l, l.center_stride, j0 + v * (kThreads * E)));
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int v = 0; v < V; ++v) r[g][v] = load_full<DT>(p[g], place<TILED>(l, l.stride, j0 + v * (kThreads * E)));
   } else {
-    const int part = clamp_part(n - j, E);
-    rc = load_part<DT>(center, at_c, part);
 #pragma unroll
-    for (int g = 0; g < G; ++g) r[g] = load_part<DT>(p[g], at, part);
-  }
-  double c[E];
-  Elem<DT>::widen(rc, c);
+    for (int v = 0; v < V; ++v) {
+      const int64_t j = j0 + v * (kThreads * E);
+      const int part = clamp_part(n - j, E);
+      rc[v] = load_part<DT>(center, place<TILED>(l, l.center_stride, j), part);
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    double x[E];
-    Elem<DT>::widen(r[g], x);
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const double d = x[i] - c[i];
-      acc[g] = __builtin_fma(d, d, acc[g]);
+      for (int g = 0; g < G; ++g) r[g][v] = load_part<DT>(p[g], place<TILED>(l, l.stride, j), part);
     }
+  }
+  double c[V][E];
+#pragma unroll
+  for (int v = 0; v < V; ++v) Elem<DT>::widen(rc[v], c[v]);
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      double x[E];
+      Elem<DT>::widen(r[g][v], x);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const double d = x[i] - c[v][i];
+        acc[g] = __builtin_fma(d, d, acc[g]);
+      }
+    }
+}
+
+// Where a peer's joined norm goes; null: not wanted.
+struct Joined {
+  const double* sq_in;  // given squares, instead of the partials
+  double* sq;           // squares
+  void* norms;          // roots, of out_dt
+  int out_dt;
+  double* shares;       // a_k, by max_norm
+  double max_norm;
+};
+// One wave: peer k's squared norm — the sum of its n partials (possibly none), or sq_in[k] — and what follows.
+__device__ inline void join_peer(const double* partials, int n, int k, const double* weights, const Joined& to) {
+  const int lane = static_cast<int>(threadIdx.x & 63);
+  double v = 0;
+  if (to.sq_in) {
+    v = global_ptr<double>(to.sq_in)[k];
+  } else {
+    v = join_strided<DLA_NORM_L2>(partials + static_cast<int64_t>(k) * n, n, lane, 64);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  }
+  if (lane != 0) return;
+  const double norm = __builtin_sqrt(v);
+  if (to.sq) global_ptr<double>(to.sq)[k] = v;
+  if (to.norms) put_norm(to.norms, k, to.out_dt, norm);
+  if (to.shares) {
+    const double share = global_ptr<double>(weights)[k] * (norm <= to.max_norm ? 1.0 : to.max_norm / norm);
+    global_ptr<double>(to.shares)[k] = __builtin_isfinite(norm) ? share : 0.0;
   }
 }
 
 // partials[k * gridDim.x + b]: workgroup b's part of || p_k - c ||^2 for the peers of group blockIdx.y.  G
-// peers are read beside one read of the centre, so the centre costs 1 / G of a peer.
-template <int G, bool TILED>
-__global__ __launch_bounds__(kThreads) void peer_norms_kernel(const Seg* segs, int count, int64_t units,
-                                                              const uint64_t* ptrs, int n_peers, Layout l,
-                                                              double* partials) {
+// peers are read beside one read of the centre, so the centre costs 1 / G of a peer.  With counters (one per
+// group), a group's last workgroup joins its peers.
+template <int G, int V, bool TILED>
+__global__ __launch_bounds__(kThreads) void peer_norms_kernel(const PutWords words, Table tab, int64_t units, Layout l,
+                                                              double* partials, uint32_t* counters, const Joined to) {
   __shared__ double lds[kWaves];
+  const TableParts parts = parts_of(tab);
+  const Seg* segs = parts.segs;
+  const uint64_t* ptrs = parts.ptrs;
+  const int count = tab.count, n_peers = tab.n_peers;
   const int64_t b = blockIdx.x, nb = gridDim.x;
   const int k0 = static_cast<int>(blockIdx.y) * G;
-  int64_t u = units * b / nb;
-  const int64_t end = units * (b + 1) / nb;
-  int t = find_seg(segs, count, u);
+  int64_t first = 0, stop = 0, n = 0;
+  int dt = 0;
+  const void* center = nullptr;
+  const void* p[G];
   double acc[G] = {};
-  while (u < end) {
-    const auto* s = const_ptr<Seg>(segs) + t;
-    const int64_t first = s->unit0, n = s->n;
-    int64_t stop = t + 1 < count ? s[1].unit0 : units;
-    if (stop > end) stop = end;
-    const void* center = s->center;
-    const void* p[G];
+  for (int64_t u = b; u < units; u += nb) {
+    if (u >= stop) {
+      const int t = find_seg<&Seg::norm_unit0>(segs, count, u);
+      const auto* s = const_ptr<Seg>(segs) + t;
+      first = s->norm_unit0;
+      n = static_cast<int64_t>(s->n_dt >> 2);
+      dt = static_cast<int>(s->n_dt & 3);
+      center = s->center;
+      stop = t + 1 < count ? s[1].norm_unit0 : units;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const int k = k0 + g < n_peers ? k0 + g : n_peers - 1;  // a spare place reads the last peer again
-      p[g] = reinterpret_cast<const void*>(const_ptr<uint64_t>(ptrs)[static_cast<int64_t>(t) * n_peers + k]);
+      for (int g = 0; g < G; ++g) {
+        const int k = k0 + g < n_peers ? k0 + g : n_peers - 1;  // a spare place reads the last peer again
+        p[g] = reinterpret_cast<const void*>(const_ptr<uint64_t>(ptrs)[static_cast<int64_t>(t) * n_peers + k]);
+      }
     }
-    switch (s->dt) {
-      case DLA_F32: for (; u < stop; ++u) peer_norm_unit<DLA_F32, G, TILED>(l, center, p, n, u - first, acc); break;
-      case DLA_BF16: for (; u < stop; ++u) peer_norm_unit<DLA_BF16, G, TILED>(l, center, p, n, u - first, acc); break;
-      case DLA_F16: for (; u < stop; ++u) peer_norm_unit<DLA_F16, G, TILED>(l, center, p, n, u - first, acc); break;
-      default: for (; u < stop; ++u) peer_norm_unit<DLA_F64, G, TILED>(l, center, p, n, u - first, acc); break;
+    switch (dt) {
+      case DLA_F32: peer_norm_unit<DLA_F32, G, V, TILED>(l, center, p, n, u - first, acc); break;
+      case DLA_BF16: peer_norm_unit<DLA_BF16, G, V, TILED>(l, center, p, n, u - first, acc); break;
+      case DLA_F16: peer_norm_unit<DLA_F16, G, V, TILED>(l, center, p, n, u - first, acc); break;
+      default: peer_norm_unit<DLA_F64, G, V, TILED>(l, center, p, n, u - first, acc); break;
     }
-    ++t;
   }
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     const double v = block_join<DLA_NORM_L2>(acc[g], lds);
-    if (threadIdx.x == 0 && k0 + g < n_peers) global_ptr<double>(partials)[(k0 + g) * nb + b] = v;
+    if (threadIdx.x == 0 && k0 + g < n_peers) publish(partials + (k0 + g) * nb + b, v);
   }
+  if (!counters || !last_to_arrive(counters)) return;
+  for (int g = static_cast<int>(threadIdx.x >> 6); g < G && k0 + g < n_peers; g += kWaves)
+    join_peer(partials, static_cast<int>(nb), k0 + g, parts.weights, to);
 }
 
-// sq[k] = the sum of peer k's partials (n of them, possibly none); norms[k] = its root.
-__global__ __launch_bounds__(kThreads) void peer_join_kernel(const double* partials, int n, double* sq, int out_dt,
-                                                             void* norms) {
-  __shared__ double lds[kWaves];
-  const int k = static_cast<int>(blockIdx.x);
-  double v = 0;
-  for (int i = threadIdx.x; i < n; i += kThreads) v += global_ptr<double>(partials)[static_cast<int64_t>(k) * n + i];
-  v = block_join<DLA_NORM_L2>(v, lds);
-  if (threadIdx.x == 0) {
-    global_ptr<double>(sq)[k] = v;
-    if (norms) put_norm(norms, k, out_dt, __builtin_sqrt(v));
-  }
+// The join as a kernel of its own: one wave per peer.
+__global__ __launch_bounds__(64) void peer_join_kernel(const PutWords words, Table tab, const double* partials, int n,
+                                                       const Joined to) {
+  join_peer(partials, n, static_cast<int>(blockIdx.x), parts_of(tab).weights, to);
 }
-
-// The peers that count, in list order, in LDS: their share a_k and their pointer for the tensor at hand.
-struct Live {
-  double* share;
-  uint64_t* ptr;
-  int* k;
-};
 
 template <int DT, int G, bool TILED>
-__device__ inline void fold_peers(const Live& live, int i0, int64_t at, int part, bool full,
-                                  const double (&c)[Elem<DT>::E], double (&acc)[Elem<DT>::E]) {
+__device__ inline void fold_peers(const uint64_t* ptrs, const double* shares, const void* center, int64_t at, int64_t at_c,
+                                  bool full, int part, const typename Average<DT>::real (&c)[Elem<DT>::E],
+                                  typename Average<DT>::real (&acc)[Elem<DT>::E]) {
+  using A = Average<DT>;
   constexpr int E = Elem<DT>::E;
   u32x4 r[G];
+  typename A::real a[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    const void* p = reinterpret_cast<const void*>(live.ptr[i0 + g]);
-    r[g] = full ? load_full<DT>(p, at) : load_part<DT>(p, at, part);
+    const double share = const_ptr<double>(shares)[g];
+    const void* p = reinterpret_cast<const void*>(const_ptr<uint64_t>(ptrs)[g]);
+    const bool counts = share != 0.0;  // a peer that does not count is not read: the centre stands in, update 0
+    p = counts ? p : center;
+    const int64_t from = TILED ? (counts ? at : at_c) : at;
+    a[g] = A::share(share);
+    r[g] = full ? load_full<DT>(p, from) : load_part<DT>(p, from, part);
   }
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    const double a = live.share[i0 + g];
-    double x[E];
+    typename A::real x[E];
     Elem<DT>::widen(r[g], x);
 #pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] = __builtin_fma(a, x[i] - c[i], acc[i]);
+    for (int i = 0; i < E; ++i) acc[i] = A::fold(a[g], A::update(x[i], c[i]), acc[i]);
   }
 }
 
 template <int DT, bool TILED>
-__device__ inline void bounded_unit(const Layout& l, const Live& live, int m, const void* center, void* out, int64_t n,
-                                    int64_t unit) {
+__device__ inline void mean_unit(const Layout& l, const uint64_t* ptrs, const double* shares, int n_peers,
+                                 const void* center, void* out, int64_t n, int64_t unit) {
+  using A = Average<DT>;
   constexpr int E = Elem<DT>::E;
-  const int64_t j = unit * (kThreads * E) + static_cast<int>(threadIdx.x) * E;
-  const int64_t at = place<TILED>(l, l.stride, j), at_c = place<TILED>(l, l.center_stride, j);
-  const bool full = (unit + 1) * (kThreads * E) <= n;
-  const int part = full ? E : clamp_part(n - j, E);
-  double c[E], acc[E] = {};
-  Elem<DT>::widen(full ? load_full<DT>(center, at_c) : load_part<DT>(center, at_c, part), c);
-  int i = 0;
-  for (; i + 8 <= m; i += 8) fold_peers<DT, 8, TILED>(live, i, at, part, full, c, acc);
-  if (i + 4 <= m) {
-    fold_peers<DT, 4, TILED>(live, i, at, part, full, c, acc);
-    i += 4;
-  }
-  if (i + 2 <= m) {
-    fold_peers<DT, 2, TILED>(live, i, at, part, full, c, acc);
-    i += 2;
-  }
-  if (i < m) fold_peers<DT, 1, TILED>(live, i, at, part, full, c, acc);
+  const bool full = (unit + 1) * (kMeanThreads * kMeanSteps * E) <= n;
+#pragma unroll 1
+  for (int step = 0; step < kMeanSteps; ++step) {
+    const int64_t j = (unit * kMeanSteps + step) * (kMeanThreads * E) + static_cast<int>(threadIdx.x) * E;
+    const int64_t at = place<TILED>(l, l.stride, j), at_c = place<TILED>(l, l.center_stride, j);
+    const int part = full ? E : clamp_part(n - j, E);
+    const u32x4 rc = full ? load_full<DT>(center, at_c) : load_part<DT>(center, at_c, part);
+    typename A::real c[E], acc[E] = {};
+    Elem<DT>::widen(rc, c);
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] += c[e];
-  store_part<DT>(out, j, part, Elem<DT>::narrow(acc));
+    for (int e = 0; e < E; ++e) c[e] = A::center(c[e]);
+    int i = 0;
+    for (; i + 8 <= n_peers; i += 8) fold_peers<DT, 8, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
+    if (i + 4 <= n_peers) {
+      fold_peers<DT, 4, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
+      i += 4;
+    }
+    if (i + 2 <= n_peers) {
+      fold_peers<DT, 2, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
+      i += 2;
+    }
+    if (i < n_peers) fold_peers<DT, 1, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
+    Elem<DT>::widen(rc, c);
+    // where the centre is not finite no peer counts, and the centre stays
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = __builtin_isfinite(c[e]) ? acc[e] + c[e] : c[e];
+    store_part<DT>(out, j, part, Elem<DT>::narrow(acc));
+  }
 }
 
-// out = round(c + sum_k a_k (p_k - c)).  Units are walked from the last to the first: what the norms read
-// last is what the caches still hold.
+// out = round(c + sum_k a_k (p_k - c)).  Units are dealt from the last to the first: what the norms read last is
+// what the caches still hold.
 template <bool TILED>
-__global__ __launch_bounds__(kThreads) void bounded_kernel(const Seg* segs, int count, int64_t units,
-                                                           const uint64_t* ptrs, const double* weights, int n_peers,
-                                                           Layout l, double max_norm, const double* sq, int out_dt,
-                                                           void* norms) {
-  extern __shared__ double lds[];
-  __shared__ int n_live;
-  Live live;
-  live.share = lds;
-  live.ptr = reinterpret_cast<uint64_t*>(lds + n_peers);
-  live.k = reinterpret_cast<int*>(lds + 2 * n_peers);
-  if (threadIdx.x < 64) {
-    int m = 0;
-    for (int k0 = 0; k0 < n_peers; k0 += 64) {
-      const int k = k0 + static_cast<int>(threadIdx.x);
-      double norm = 0, share = 0;
-      if (k < n_peers) {
-        norm = __builtin_sqrt(global_ptr<double>(sq)[k]);
-        share = global_ptr<double>(weights)[k] * (norm <= max_norm ? 1.0 : max_norm / norm);
-        if (blockIdx.x == 0 && norms) put_norm(norms, k, out_dt, norm);
-      }
-      const bool counts = k < n_peers && __builtin_isfinite(norm) && share != 0.0;
-      const uint64_t mask = __ballot(counts);
-      if (counts) {
-        const int at = m + __popcll(mask & ((uint64_t{1} << threadIdx.x) - 1));
-        live.share[at] = share;
-        live.k[at] = k;
-      }
-      m += __popcll(mask);
-    }
-    if (threadIdx.x == 0) n_live = m;
-  }
-  __syncthreads();
-  const int m = __builtin_amdgcn_readfirstlane(n_live);
-  const int64_t b = blockIdx.x, nb = gridDim.x;
-  const int64_t begin = units * b / nb;
-  int64_t u = units * (b + 1) / nb;
-  if (u == begin) return;
-  int t = find_seg(segs, count, u - 1);
-  while (u > begin) {
+__global__ __launch_bounds__(kMeanThreads) void bounded_kernel(const PutWords words, Table tab, int64_t units,
+                                                               const double* shares, Layout l) {
+  const TableParts parts = parts_of(tab);
+  const Seg* segs = parts.segs;
+  const uint64_t* ptrs = parts.ptrs;
+  const int count = tab.count, n_peers = tab.n_peers;
+  for (int64_t u = units - 1 - blockIdx.x; u >= 0; u -= gridDim.x) {
+    const int t = find_seg<&Seg::mean_unit0>(segs, count, u);
     const auto* s = const_ptr<Seg>(segs) + t;
-    const int64_t first = s->unit0, n = s->n;
-    const int64_t stop = first > begin ? first : begin;
+    const int64_t first = s->mean_unit0, n = static_cast<int64_t>(s->n_dt >> 2);
     const void* center = s->center;
     void* out = s->out;
-    for (int i = threadIdx.x; i < m; i += kThreads)
-      live.ptr[i] = global_ptr<uint64_t>(ptrs)[static_cast<int64_t>(t) * n_peers + live.k[i]];
-    __syncthreads();
-    switch (s->dt) {
-      case DLA_F32: for (; u > stop; --u) bounded_unit<DLA_F32, TILED>(l, live, m, center, out, n, u - 1 - first); break;
-      case DLA_BF16: for (; u > stop; --u) bounded_unit<DLA_BF16, TILED>(l, live, m, center, out, n, u - 1 - first); break;
-      case DLA_F16: for (; u > stop; --u) bounded_unit<DLA_F16, TILED>(l, live, m, center, out, n, u - 1 - first); break;
-      default: for (; u > stop; --u) bounded_unit<DLA_F64, TILED>(l, live, m, center, out, n, u - 1 - first); break;
+    const uint64_t* mine = ptrs + static_cast<int64_t>(t) * n_peers;
+    switch (s->n_dt & 3) {
+      case DLA_F32: mean_unit<DLA_F32, TILED>(l, mine, shares, n_peers, center, out, n, u - first); break;
+      case DLA_BF16: mean_unit<DLA_BF16, TILED>(l, mine, shares, n_peers, center, out, n, u - first); break;
+      case DLA_F16: mean_unit<DLA_F16, TILED>(l, mine, shares, n_peers, center, out, n, u - first); break;
+      default: mean_unit<DLA_F64, TILED>(l, mine, shares, n_peers, center, out, n, u - first); break;
     }
-    __syncthreads();  // live.ptr is filled again for the next tensor
-    --t;
   }
 }
 
@@ -620,41 +748,38 @@ bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(
 // No element count here exceeds this: 2^56 bytes, far beyond any device, keeps every product below in 64 bits.
 constexpr int64_t kMostElems = int64_t{1} << 53;
 
-// The launches a list of tensors takes: tensors [begin, end) of `order` (the non-empty ones), `units` units
-// on `blocks` workgroups whose partials start at `partial0`.
+// The launches a list of tensors takes: tensors [begin, end) of `order` (the non-empty ones), `units` units on
+// `blocks` workgroups.
 struct ListLaunch {
   int begin, end;
   uint32_t units;
-  int blocks, partial0;
+  int blocks;
 };
 
-int64_t list_units(int dt, int64_t n) {
-  const int64_t per = kUnitBytes / elem_bytes(dt);
+int64_t list_units(int dt, int64_t n, int vec) {
+  const int64_t per = unit_bytes(vec) / elem_bytes(dt);
   return (n + per - 1) / per;
 }
 
-bool plan_list(const std::vector<int>& order, const int* dtypes, const int64_t* numels, int per_launch, int most_blocks,
-               std::vector<ListLaunch>* out, int* partials) {
+// `most` workgroups in all, shared by the launches as their units are, or (0) one per unit.
+bool plan_list(const std::vector<int>& order, const int* dtypes, const int64_t* numels, int vec, int per_launch, int64_t most,
+               std::vector<ListLaunch>* out) {
   int64_t total = 0;
-  for (int t : order) total += list_units(dtypes[t], numels[t]);
-  int p0 = 0;
+  for (int t : order) total += list_units(dtypes[t], numels[t], vec);
   for (size_t i = 0; i < order.size(); i += per_launch) {
     const int end = static_cast<int>(std::min(order.size(), i + per_launch));
     int64_t units = 0;
-    for (int q = static_cast<int>(i); q < end; ++q) units += list_units(dtypes[order[q]], numels[order[q]]);
+    for (int q = static_cast<int>(i); q < end; ++q) units += list_units(dtypes[order[q]], numels[order[q]], vec);
     if (units > 0xffffffffll) return false;
-    int64_t blocks = std::min<int64_t>(units, most_blocks);
-    if (total > units) blocks = std::max<int64_t>(1, std::min<int64_t>(blocks, most_blocks * units / total));
-    out->push_back({static_cast<int>(i), end, static_cast<uint32_t>(units), static_cast<int>(blocks), p0});
-    p0 += static_cast<int>(blocks);
+    const int64_t share = most ? std::max<int64_t>(1, most * units / total) : 0x7fffffff;
+    out->push_back({static_cast<int>(i), end, static_cast<uint32_t>(units), static_cast<int>(std::min(units, share))});
   }
-  *partials = p0;
   return true;
 }
 
 template <int M>
 void fill_list(TensorList<M>* tab, const ListLaunch& l, const std::vector<int>& order, const int* dtypes,
-               const void* const* tensors, const int64_t* numels) {
+               const void* const* tensors, const int64_t* numels, int vec) {
   std::memset(tab, 0, sizeof(*tab));
   uint32_t u = 0;
   for (int q = l.begin; q < l.end; ++q) {
@@ -662,7 +787,7 @@ void fill_list(TensorList<M>* tab, const ListLaunch& l, const std::vector<int>& 
     tab->p[i] = tensors[t];
     tab->n_dt[i] = static_cast<uint64_t>(numels[t]) * 4 + static_cast<uint64_t>(dtypes[t]);
     tab->unit0[i] = u;
-    u += static_cast<uint32_t>(list_units(dtypes[t], numels[t]));
+    u += static_cast<uint32_t>(list_units(dtypes[t], numels[t], vec));
   }
 }
 
@@ -707,100 +832,140 @@ bool meets(const std::vector<Span>& outs, const Span& s, const Span& own) {
   return it != outs.begin() && std::prev(it)->end > s.begin;
 }
 
-int norm_impl(int n_tensors, const int* dtypes, const void* const* tensors, const int64_t* numels, int norm, int out_dtype,
-              void* out, void* workspace, int64_t workspace_bytes, void* stream) {
-  std::vector<int> order;
-  if (int rc = check_list("dla_norm", n_tensors, dtypes, tensors, numels, norm, &order)) return rc;
-  if (out && ((out_dtype != DLA_F32 && out_dtype != DLA_F64) || !aligned_to(out, elem_bytes(out_dtype))))
-    return fail(DLA_E_INVALID, "dla_norm: out must be an aligned F32 or F64 value");
-  if (!workspace || !aligned_to(workspace, 8) || workspace_bytes < dla_norm_workspace(n_tensors))
-    return fail(DLA_E_INVALID, "dla_norm: workspace is null, not aligned or smaller than dla_norm_workspace");
+// f(norm, nt) with both as constants.
+template <class F>
+void with_norm(int norm, bool nt, F f) {
+  using std::integral_constant;
+  const auto by_nt = [&](auto p) {
+    if (nt) f(p, std::true_type{});
+    else f(p, std::false_type{});
+  };
+  if (norm == DLA_NORM_L2) by_nt(integral_constant<int, DLA_NORM_L2>{});
+  else if (norm == DLA_NORM_L1) by_nt(integral_constant<int, DLA_NORM_L1>{});
+  else by_nt(integral_constant<int, DLA_NORM_INF>{});
+}
+
+// The workspace of a list's norm: the joined norm, then the partials.
+int norm_launches(const char* what, const std::vector<int>& order, const int* dtypes, const void* const* tensors,
+                  const int64_t* numels, int norm, bool nt, int out_dtype, void* out, void* counter, double* workspace,
+                  int* n_partials, hipStream_t s) {
   std::vector<ListLaunch> launches;
-  int n_partials = 0;
-  if (!plan_list(order, dtypes, numels, kNormTensors, kMaxPartials, &launches, &n_partials))
-    return fail(DLA_E_INVALID, "dla_norm: too many elements");
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  double* partials = static_cast<double*>(workspace);
+  if (!plan_list(order, dtypes, numels, kNormVec, kNormTensors, kMaxPartials, &launches))
+    return fail(DLA_E_INVALID, std::string(what) + ": too many elements");
+  double* partials = workspace + 1;
+  *n_partials = 0;
+  for (const ListLaunch& l : launches) *n_partials += l.blocks;
+  double* to = partials;
   for (const ListLaunch& l : launches) {
     TensorList<kNormTensors> tab;
-    fill_list(&tab, l, order, dtypes, tensors, numels);
+    fill_list(&tab, l, order, dtypes, tensors, numels, kNormVec);
     const dim3 grid(static_cast<unsigned>(l.blocks));
     const int count = l.end - l.begin;
-    double* to = partials + l.partial0;
-    if (norm == DLA_NORM_L2) hipLaunchKernelGGL((norm_kernel<DLA_NORM_L2>), grid, dim3(kThreads), 0, s, tab, count, l.units, to);
-    else if (norm == DLA_NORM_L1) hipLaunchKernelGGL((norm_kernel<DLA_NORM_L1>), grid, dim3(kThreads), 0, s, tab, count, l.units, to);
-    else hipLaunchKernelGGL((norm_kernel<DLA_NORM_INF>), grid, dim3(kThreads), 0, s, tab, count, l.units, to);
-    if (hipError_t e = hipGetLastError()) return hip_fail("dla_norm", e);
-  }
-  if (out) {
-    if (norm == DLA_NORM_L2) hipLaunchKernelGGL((norm_join_kernel<DLA_NORM_L2>), dim3(1), dim3(kThreads), 0, s, partials, n_partials, out_dtype, out);
-    else if (norm == DLA_NORM_L1) hipLaunchKernelGGL((norm_join_kernel<DLA_NORM_L1>), dim3(1), dim3(kThreads), 0, s, partials, n_partials, out_dtype, out);
-    else hipLaunchKernelGGL((norm_join_kernel<DLA_NORM_INF>), dim3(1), dim3(kThreads), 0, s, partials, n_partials, out_dtype, out);
-    if (hipError_t e = hipGetLastError()) return hip_fail("dla_norm", e);
+    uint32_t* last = &l == &launches.back() ? static_cast<uint32_t*>(counter) : nullptr;
+    with_norm(norm, nt, [&](auto p, auto stream_once) {
+      hipLaunchKernelGGL((norm_kernel<p(), stream_once()>), grid, dim3(kThreads), 0, s, tab, count, l.units, to, last,
+                         partials, *n_partials, workspace, out_dtype, out);
+    });
+    to += l.blocks;
+    if (hipError_t e = hipGetLastError()) return hip_fail(what, e);
   }
   return DLA_OK;
 }
 
-int norm_scale_impl(int n_tensors, const int* dtypes, const void* const* tensors, void* const* outs, const int64_t* numels,
-                    int norm, double max_norm, double eps, int out_dtype, void* norm_out, const void* workspace,
-                    int64_t workspace_bytes, void* stream) {
-  std::vector<int> order;
-  if (int rc = check_list("dla_norm_scale", n_tensors, dtypes, tensors, numels, norm, &order)) return rc;
-  if (!(max_norm >= 0) || !(eps >= 0)) return fail(DLA_E_INVALID, "dla_norm_scale: max_norm and eps must be >= 0");
-  if (norm_out && ((out_dtype != DLA_F32 && out_dtype != DLA_F64) || !aligned_to(norm_out, elem_bytes(out_dtype))))
-    return fail(DLA_E_INVALID, "dla_norm_scale: norm_out must be an aligned F32 or F64 value");
+// The joined norm from the partials, where no counter did it (none: the norm of nothing, 0).
+int join_launch(const char* what, int norm, const double* workspace, int n_partials, int out_dtype, void* out, hipStream_t s) {
+  const double* partials = workspace + 1;
+  with_norm(norm, true, [&](auto p, auto) {
+    hipLaunchKernelGGL((norm_join_kernel<p()>), dim3(1), dim3(kThreads), 0, s, partials, n_partials, out_dtype, out);
+  });
+  if (hipError_t e = hipGetLastError()) return hip_fail(what, e);
+  return DLA_OK;
+}
+
+int check_norm_memory(const char* what, int n_tensors, int out_dtype, const void* out, const void* counter,
+                      const void* workspace, int64_t workspace_bytes) {
+  const std::string w(what);
+  if (out && ((out_dtype != DLA_F32 && out_dtype != DLA_F64) || !aligned_to(out, elem_bytes(out_dtype))))
+    return fail(DLA_E_INVALID, w + ": the norm goes to an aligned F32 or F64 value");
+  if (!aligned_to(counter, 4)) return fail(DLA_E_INVALID, w + ": counter is not aligned");
   if (!workspace || !aligned_to(workspace, 8) || workspace_bytes < dla_norm_workspace(n_tensors))
-    return fail(DLA_E_INVALID, "dla_norm_scale: workspace is null, not aligned or smaller than dla_norm_workspace");
-  if (!order.empty() && !outs) return fail(DLA_E_INVALID, "dla_norm_scale: null outs array");
+    return fail(DLA_E_INVALID, w + ": workspace is null, not aligned or smaller than dla_norm_workspace");
+  return DLA_OK;
+}
+
+int norm_impl(int n_tensors, const int* dtypes, const void* const* tensors, const int64_t* numels, int norm, int out_dtype,
+              void* out, void* counter, void* workspace, int64_t workspace_bytes, void* stream) {
+  std::vector<int> order;
+  if (int rc = check_list("dla_norm", n_tensors, dtypes, tensors, numels, norm, &order)) return rc;
+  if (!out) return fail(DLA_E_INVALID, "dla_norm: null out");
+  if (int rc = check_norm_memory("dla_norm", n_tensors, out_dtype, out, counter, workspace, workspace_bytes)) return rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  double* ws = static_cast<double*>(workspace);
+  int n_partials = 0;
+  if (int rc = norm_launches("dla_norm", order, dtypes, tensors, numels, norm, true, out_dtype, out, counter, ws, &n_partials, s)) return rc;
+  return counter && n_partials > 0 ? DLA_OK : join_launch("dla_norm", norm, ws, n_partials, out_dtype, out, s);
+}
+
+int norm_clip_impl(int n_tensors, const int* dtypes, const void* const* tensors, void* const* outs, const int64_t* numels,
+                   int norm, double max_norm, double eps, int out_dtype, void* norm_out, void* counter, void* workspace,
+                   int64_t workspace_bytes, void* stream) {
+  std::vector<int> order;
+  if (int rc = check_list("dla_norm_clip", n_tensors, dtypes, tensors, numels, norm, &order)) return rc;
+  if (!(max_norm >= 0) || !(eps >= 0)) return fail(DLA_E_INVALID, "dla_norm_clip: max_norm and eps must be >= 0");
+  if (int rc = check_norm_memory("dla_norm_clip", n_tensors, out_dtype, norm_out, counter, workspace, workspace_bytes)) return rc;
+  if (!order.empty() && !outs) return fail(DLA_E_INVALID, "dla_norm_clip: null outs array");
   std::vector<Span> spans;
   bool in_place = true;
   for (int t : order) {
     if (!outs[t] || !aligned_to(outs[t], elem_bytes(dtypes[t])))
-      return fail(DLA_E_INVALID, "dla_norm_scale: out " + std::to_string(t) + " is null or not aligned to its elements");
+      return fail(DLA_E_INVALID, "dla_norm_clip: out " + std::to_string(t) + " is null or not aligned to its elements");
     spans.push_back(span_of(outs[t], numels[t], elem_bytes(dtypes[t])));
     in_place = in_place && outs[t] == tensors[t];
   }
   const std::vector<Span> own = spans;
-  if (!disjoint(&spans)) return fail(DLA_E_ALIAS, "dla_norm_scale: two outputs overlap");
+  if (!disjoint(&spans)) return fail(DLA_E_ALIAS, "dla_norm_clip: two outputs overlap");
   for (size_t q = 0; q < order.size() && !in_place; ++q)
     if (meets(spans, span_of(tensors[order[q]], numels[order[q]], elem_bytes(dtypes[order[q]])), own[q]))
-      return fail(DLA_E_ALIAS, "dla_norm_scale: tensor " + std::to_string(order[q]) + " overlaps an output that is not its own");
-  std::vector<ListLaunch> parts, launches;
-  int n_partials = 0, unused = 0;
-  if (!plan_list(order, dtypes, numels, kNormTensors, kMaxPartials, &parts, &n_partials) ||
-      !plan_list(order, dtypes, numels, kScaleTensors, 2 * kMaxPartials, &launches, &unused))
-    return fail(DLA_E_INVALID, "dla_norm_scale: too many elements");
+      return fail(DLA_E_ALIAS, "dla_norm_clip: tensor " + std::to_string(order[q]) + " overlaps an output that is not its own");
+  std::vector<ListLaunch> launches;
+  int n_partials = 0;
+  if (!plan_list(order, dtypes, numels, kScaleVec, kScaleTensors, 0, &launches))
+    return fail(DLA_E_INVALID, "dla_norm_clip: too many elements");
+  // What the Infinity Cache (256 MB) can hold is kept in the caches for the second read; more streams past them
+  // (us, kept / streamed: 21 M bf16 27.4 / 30.8, 40 M f32 79.0 / 82.3; 0.87 G bf16 933 / 889)
+  int64_t bytes = 0;
+  for (int t : order) bytes += numels[t] * elem_bytes(dtypes[t]);
+  const bool nt = bytes > (int64_t{256} << 20);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const double* partials = static_cast<const double*>(workspace);
+  double* ws = static_cast<double*>(workspace);
+  if (int rc = norm_launches("dla_norm_clip", order, dtypes, tensors, numels, norm, nt, out_dtype, nullptr, counter, ws, &n_partials, s)) return rc;
+  if (launches.empty()) return norm_out ? join_launch("dla_norm_clip", norm, ws, 0, out_dtype, norm_out, s) : DLA_OK;
+  if (!counter)
+    if (int rc = join_launch("dla_norm_clip", norm, ws, n_partials, DLA_F64, ws, s)) return rc;
   for (const ListLaunch& l : launches) {
     TensorsInOut<kScaleTensors> tab;
-    fill_list(&tab.in, l, order, dtypes, tensors, numels);
+    fill_list(&tab.in, l, order, dtypes, tensors, numels, kScaleVec);
     std::memset(tab.out, 0, sizeof(tab.out));
     for (int q = l.begin; q < l.end; ++q) tab.out[q - l.begin] = outs[order[q]];
     const dim3 grid(static_cast<unsigned>(l.blocks));
     const int count = l.end - l.begin, inp = in_place ? 1 : 0;
     void* no = l.begin == 0 ? norm_out : nullptr;
-    if (norm == DLA_NORM_L2) hipLaunchKernelGGL((norm_scale_kernel<DLA_NORM_L2>), grid, dim3(kThreads), 0, s, tab, count, l.units, partials, n_partials, max_norm, eps, inp, out_dtype, no);
-    else if (norm == DLA_NORM_L1) hipLaunchKernelGGL((norm_scale_kernel<DLA_NORM_L1>), grid, dim3(kThreads), 0, s, tab, count, l.units, partials, n_partials, max_norm, eps, inp, out_dtype, no);
-    else hipLaunchKernelGGL((norm_scale_kernel<DLA_NORM_INF>), grid, dim3(kThreads), 0, s, tab, count, l.units, partials, n_partials, max_norm, eps, inp, out_dtype, no);
-    if (hipError_t e = hipGetLastError()) return hip_fail("dla_norm_scale", e);
-  }
-  if (launches.empty() && norm_out) {  // nothing to scale: the norm of nothing is 0
-    hipLaunchKernelGGL((norm_join_kernel<DLA_NORM_L1>), dim3(1), dim3(kThreads), 0, s, partials, 0, out_dtype, norm_out);
-    if (hipError_t e = hipGetLastError()) return hip_fail("dla_norm_scale", e);
+    if (nt) hipLaunchKernelGGL((norm_scale_kernel<true>), grid, dim3(kThreads), 0, s, tab, count, l.units, ws, max_norm, eps, inp, out_dtype, no);
+    else hipLaunchKernelGGL((norm_scale_kernel<false>), grid, dim3(kThreads), 0, s, tab, count, l.units, ws, max_norm, eps, inp, out_dtype, no);
+    if (hipError_t e = hipGetLastError()) return hip_fail("dla_norm_clip", e);
   }
   return DLA_OK;
 }
 
 // ------------------------------------------------------------------ peers, host side
 constexpr int kPeerBlocks = 1024;  // workgroups of the norms: 4 per CU
-constexpr int kMostPeers = 2048;   // their shares and pointers in LDS: 20 bytes each
+constexpr int kMostPeers = 2048;
 
 int64_t peer_table_words(int64_t n_tensors, int64_t n_peers) {
   return n_tensors * static_cast<int64_t>(sizeof(Seg) / 8) + n_tensors * n_peers + n_peers;
 }
 int64_t peer_workspace_bytes(int64_t n_tensors, int64_t n_peers) {
-  return (peer_table_words(n_tensors, n_peers) + n_peers /* sq */ + n_peers * kPeerBlocks) * 8;
+  return (peer_table_words(n_tensors, n_peers) + n_peers /* shares */ + n_peers * kPeerBlocks) * 8;
 }
 
 struct Round {  // a round's arguments, as the entry points give them
@@ -856,48 +1021,85 @@ int check_round(const char* what, const Round& r, std::vector<int>* order) {
   return DLA_OK;
 }
 
-// Writes the round's table into `dst` (device); *units: the units of all tensors.
-int put_table(const char* what, const Round& r, const std::vector<int>& order, uint64_t* dst, int64_t* units, hipStream_t s) {
+int64_t units_of(int64_t n, int dt, int unit_bytes) {
+  const int64_t per = unit_bytes / elem_bytes(dt);
+  return (n + per - 1) / per;
+}
+
+// The round's table: in `words` if it fits there, else in the workspace.
+int make_table(const char* what, const Round& r, const std::vector<int>& order, int norm_unit, void* table_host,
+               int64_t table_host_bytes, uint64_t* workspace, PutWords* words, Table* tab, int64_t* norm_units,
+               int64_t* mean_units, hipStream_t s) {
   const int m = static_cast<int>(order.size());
-  std::vector<uint64_t> words(static_cast<size_t>(peer_table_words(m, r.n_peers)));
-  Seg* segs = reinterpret_cast<Seg*>(words.data());
-  uint64_t* ptrs = words.data() + m * (sizeof(Seg) / 8);
-  int64_t u = 0;
+  const int64_t n_words = peer_table_words(m, r.n_peers);
+  const bool here = n_words <= kPutWords;
+  const bool host = !here && table_host && table_host_bytes >= n_words * 8 && aligned_to(table_host, 8);
+  std::vector<uint64_t> built(here || host ? 0 : static_cast<size_t>(n_words));
+  uint64_t* to = here ? words->w : host ? static_cast<uint64_t*>(table_host) : built.data();
+  Seg* segs = reinterpret_cast<Seg*>(to);
+  uint64_t* ptrs = to + m * (sizeof(Seg) / 8);
+  int64_t un = 0, um = 0;
   for (int q = 0; q < m; ++q) {
-    const int t = order[q];
-    segs[q] = {u, r.numels[t], r.centers[t], r.outs ? r.outs[t] : nullptr, r.dtypes[t]};
+    const int t = order[q], dt = r.dtypes[t];
+    segs[q] = {un, um, static_cast<uint64_t>(r.numels[t]) * 4 + static_cast<uint64_t>(dt), r.centers[t], r.outs ? r.outs[t] : nullptr};
     for (int k = 0; k < r.n_peers; ++k)
       ptrs[static_cast<int64_t>(q) * r.n_peers + k] = reinterpret_cast<uint64_t>(r.peers[static_cast<int64_t>(t) * r.n_peers + k]);
-    const int64_t per = kPeerUnit / elem_bytes(r.dtypes[t]);
-    u += (r.numels[t] + per - 1) / per;
+    un += units_of(r.numels[t], dt, norm_unit);
+    um += units_of(r.numels[t], dt, kMeanUnit);
   }
   if (r.weights) std::memcpy(ptrs + static_cast<int64_t>(m) * r.n_peers, r.weights, sizeof(double) * r.n_peers);
-  for (size_t i = 0; i < words.size(); i += kPutWords) {
-    PutWords blob;
-    const int n = static_cast<int>(std::min<size_t>(kPutWords, words.size() - i));
-    std::memcpy(blob.w, words.data() + i, sizeof(uint64_t) * n);
-    hipLaunchKernelGGL(put_kernel, dim3(1), dim3(512), 0, s, blob, dst + i, n);
+  *tab = {here ? nullptr : workspace, m, r.n_peers};
+  *norm_units = un;
+  *mean_units = um;
+  if (host) {
+    hipLaunchKernelGGL(fetch_kernel, dim3(static_cast<unsigned>((n_words + kThreads - 1) / kThreads)), dim3(kThreads), 0, s,
+                       to, workspace, n_words);
     if (hipError_t e = hipGetLastError()) return hip_fail(what, e);
   }
-  *units = u;
+  for (size_t i = 0; i < built.size(); i += kPutWords) {
+    PutWords blob;
+    const int n = static_cast<int>(std::min<size_t>(kPutWords, built.size() - i));
+    std::memcpy(blob.w, built.data() + i, sizeof(uint64_t) * n);
+    hipLaunchKernelGGL(put_kernel, dim3(1), dim3(512), 0, s, blob, workspace + i, n);
+    if (hipError_t e = hipGetLastError()) return hip_fail(what, e);
+  }
   return DLA_OK;
 }
 
+struct NormLaunch {
+  const PutWords& words;
+  Table tab;
+  bool tiled, wide;  // wide: kPeerVec loads of one peer in a row
+  dim3 grid;
+  hipStream_t s;
+  int64_t units;
+  Layout l;
+  double* partials;
+  uint32_t* counters;
+  const Joined& to;
+};
+template <int G, int V, bool TILED>
+void launch_peer_norms(const NormLaunch& a) {
+  hipLaunchKernelGGL((peer_norms_kernel<G, V, TILED>), a.grid, dim3(kThreads), 0, a.s, a.words, a.tab, a.units, a.l, a.partials,
+                     a.counters, a.to);
+}
 template <int G>
-void launch_peer_norms(bool tiled, dim3 grid, hipStream_t s, const Seg* segs, int m, int64_t units, const uint64_t* ptrs,
-                       int n, const Layout& l, double* partials) {
-  if (tiled) hipLaunchKernelGGL((peer_norms_kernel<G, true>), grid, dim3(kThreads), 0, s, segs, m, units, ptrs, n, l, partials);
-  else hipLaunchKernelGGL((peer_norms_kernel<G, false>), grid, dim3(kThreads), 0, s, segs, m, units, ptrs, n, l, partials);
+void launch_peer_norms(const NormLaunch& a) {
+  if (a.tiled) launch_peer_norms<G, 1, true>(a);
+  else if (a.wide) launch_peer_norms<G, kPeerVec, false>(a);
+  else launch_peer_norms<G, 1, false>(a);
 }
 
-// The norms (sq != null, or outs == null), then the average (outs != null), of one round.
+// The norms (no sq_in), then the average (outs != null), of one round.
 int round_impl(const char* what, const Round& r, double max_norm, const double* sq_in, double* sq_out, int out_dtype,
-               void* norms, void* workspace, int64_t workspace_bytes, void* stream) {
+               void* norms, void* counters, void* table_host, int64_t table_host_bytes, void* workspace,
+               int64_t workspace_bytes, void* stream) {
   std::vector<int> order;
   if (int rc = check_round(what, r, &order)) return rc;
   const std::string w(what);
   if (norms && ((out_dtype != DLA_F32 && out_dtype != DLA_F64) || !aligned_to(norms, elem_bytes(out_dtype))))
     return fail(DLA_E_INVALID, w + ": norms must be aligned F32 or F64 values");
+  if (!aligned_to(counters, 4)) return fail(DLA_E_INVALID, w + ": counters are not aligned");
   if (r.outs && !r.weights) return fail(DLA_E_INVALID, w + ": null weights");
   if (r.outs && !(max_norm >= 0)) return fail(DLA_E_INVALID, w + ": max_norm must be >= 0");
   if (!workspace || !aligned_to(workspace, 8) || workspace_bytes < peer_workspace_bytes(r.n_tensors, r.n_peers))
@@ -905,44 +1107,55 @@ int round_impl(const char* what, const Round& r, double max_norm, const double* 
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int m = static_cast<int>(order.size()), n = r.n_peers;
   uint64_t* table = static_cast<uint64_t*>(workspace);
-  int64_t units = 0;
-  if (m > 0)
-    if (int rc = put_table(what, r, order, table, &units, s)) return rc;
-  const Seg* segs = reinterpret_cast<const Seg*>(table);
-  const uint64_t* ptrs = table + m * (sizeof(Seg) / 8);
-  const double* weights = reinterpret_cast<const double*>(ptrs + static_cast<int64_t>(m) * n);
-  double* sq = sq_out ? sq_out : reinterpret_cast<double*>(table + peer_table_words(r.n_tensors, n));
-  double* partials = reinterpret_cast<double*>(table + peer_table_words(r.n_tensors, n) + n);
-  if (!sq_in) {
-    int64_t blocks = 0;
-    if (m > 0) {
-      // peers beside one read of the centre: 8 at most (their loads are all in flight), groups of equal size
-      const int groups = (n + 7) / 8, g = (n + groups - 1) / groups;
-      blocks = std::min<int64_t>(units, std::max<int64_t>(1, kPeerBlocks / groups));
-      const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((n + g - 1) / g));
-      switch (g) {
-        case 1: launch_peer_norms<1>(r.tiled, grid, s, segs, m, units, ptrs, n, r.layout, partials); break;
-        case 2: launch_peer_norms<2>(r.tiled, grid, s, segs, m, units, ptrs, n, r.layout, partials); break;
-        case 3: launch_peer_norms<3>(r.tiled, grid, s, segs, m, units, ptrs, n, r.layout, partials); break;
-        case 4: launch_peer_norms<4>(r.tiled, grid, s, segs, m, units, ptrs, n, r.layout, partials); break;
-        case 5: launch_peer_norms<5>(r.tiled, grid, s, segs, m, units, ptrs, n, r.layout, partials); break;
-        case 6: launch_peer_norms<6>(r.tiled, grid, s, segs, m, units, ptrs, n, r.layout, partials); break;
-        case 7: launch_peer_norms<7>(r.tiled, grid, s, segs, m, units, ptrs, n, r.layout, partials); break;
-        default: launch_peer_norms<8>(r.tiled, grid, s, segs, m, units, ptrs, n, r.layout, partials); break;
-      }
-      if (hipError_t e = hipGetLastError()) return hip_fail(what, e);
+  const bool wide = !r.tiled;
+  int64_t norm_units = 0, mean_units = 0;
+  PutWords words;
+  Table tab;
+  if (int rc = make_table(what, r, order, wide ? kNormUnit * kPeerVec : kNormUnit, table_host, table_host_bytes, table, &words,
+                          &tab, &norm_units, &mean_units, s))
+    return rc;
+  double* shares = reinterpret_cast<double*>(table + peer_table_words(r.n_tensors, n));
+  double* partials = shares + n;
+  const Joined to = {sq_in, sq_out, norms, out_dtype, r.outs ? shares : nullptr, max_norm};
+  int64_t blocks = 0;
+  if (!sq_in && m > 0) {
+    // peers beside one read of the centre: 8 at most (their loads are all in flight), groups of equal size
+    const int groups = (n + 7) / 8, g = (n + groups - 1) / groups;
+    blocks = std::min<int64_t>(norm_units, std::max<int64_t>(1, kPeerBlocks / groups));
+    // large rounds join in a kernel of its own: its launch hides behind the round, the last workgroup's join does
+    // not (us, apart / in the last workgroup: 8 x 25 M f32 138.6 / 141.6; but 2 x 85 K f32 with the average 15.5 / 12.7)
+    if (blocks * groups > kPeerBlocks / 2) counters = nullptr;
+    const NormLaunch a = {words, tab, r.tiled, wide, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>((n + g - 1) / g)), s,
+                          norm_units, r.layout, partials, static_cast<uint32_t*>(counters), to};
+    switch (g) {
+      case 1: launch_peer_norms<1>(a); break;
+      case 2: launch_peer_norms<2>(a); break;
+      case 3: launch_peer_norms<3>(a); break;
+      case 4: launch_peer_norms<4>(a); break;
+      case 5: launch_peer_norms<5>(a); break;
+      case 6: launch_peer_norms<6>(a); break;
+      case 7: launch_peer_norms<7>(a); break;
+      default: launch_peer_norms<8>(a); break;
     }
-    hipLaunchKernelGGL(peer_join_kernel, dim3(static_cast<unsigned>(n)), dim3(kThreads), 0, s, partials,
-                       static_cast<int>(blocks), sq, out_dtype, norms);
     if (hipError_t e = hipGetLastError()) return hip_fail(what, e);
   }
-  if (!r.outs) return DLA_OK;
-  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(units, 2 * kPeerBlocks));
-  const size_t lds = static_cast<size_t>(n) * 20;
-  const double* from = sq_in ? sq_in : sq;
-  void* put = sq_in ? norms : nullptr;
-  if (r.tiled) hipLaunchKernelGGL((bounded_kernel<true>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), lds, s, segs, m, units, ptrs, weights, n, r.layout, max_norm, from, out_dtype, put);
-  else hipLaunchKernelGGL((bounded_kernel<false>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), lds, s, segs, m, units, ptrs, weights, n, r.layout, max_norm, from, out_dtype, put);
+  if (!counters || blocks == 0) {
+    hipLaunchKernelGGL(peer_join_kernel, dim3(static_cast<unsigned>(n)), dim3(64), 0, s, words, tab, partials,
+                       static_cast<int>(blocks), to);
+    if (hipError_t e = hipGetLastError()) return hip_fail(what, e);
+  }
+  if (!r.outs || m == 0) return DLA_OK;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(mean_units, 0x7fffffff)));
+  // One wave per workgroup and 8 + 1 loads in flight per wave: beyond some 100 KB in flight per CU more waves only
+  // keep more DRAM rows open at once.  Rounds of 8 peers and more that read over the Infinity Cache's 256 MB run
+  // 14 waves per CU, by reserving LDS that nothing reads (us, 14 / uncapped: 8 x 25 M f32 157 / 165, 16 x ResNet-34
+  // bf16 128.7 / 130.9, 128 x 2.7 M bf16 127.7 / 130.3); fewer peers lose by it (2 x 25 M f32 74 / 65), smaller
+  // rounds tie (32 x 1.7 M f32 43.3 / 43.0).
+  int64_t bytes = 0;
+  for (int t : order) bytes += r.numels[t] * elem_bytes(r.dtypes[t]) * (n + 1);
+  const int lds = n >= 8 && bytes > (int64_t{256} << 20) ? 160 * 1024 / 14 : 0;
+  if (r.tiled) hipLaunchKernelGGL((bounded_kernel<true>), grid, dim3(kMeanThreads), lds, s, words, tab, mean_units, shares, r.layout);
+  else hipLaunchKernelGGL((bounded_kernel<false>), grid, dim3(kMeanThreads), lds, s, words, tab, mean_units, shares, r.layout);
   if (hipError_t e = hipGetLastError()) return hip_fail(what, e);
   return DLA_OK;
 }
@@ -1004,22 +1217,22 @@ extern "C" {
 
 int64_t dla_norm_workspace(int n_tensors) {
   if (n_tensors < 0) return 0;
-  return 8 * (static_cast<int64_t>(kMaxPartials) + n_tensors / kNormTensors + 1);
+  return 8 * (static_cast<int64_t>(1) + kMaxPartials + n_tensors / kNormTensors + 1);
 }
 
 int dla_norm(int n_tensors, const int* dtypes, const void* const* tensors, const int64_t* numels, int norm, int out_dtype,
-             void* out, void* workspace, int64_t workspace_bytes, void* stream) {
+             void* out, void* counter, void* workspace, int64_t workspace_bytes, void* stream) {
   return guarded("dla_norm", [&] {
-    return norm_impl(n_tensors, dtypes, tensors, numels, norm, out_dtype, out, workspace, workspace_bytes, stream);
+    return norm_impl(n_tensors, dtypes, tensors, numels, norm, out_dtype, out, counter, workspace, workspace_bytes, stream);
   });
 }
 
-int dla_norm_scale(int n_tensors, const int* dtypes, const void* const* tensors, void* const* outs, const int64_t* numels,
-                   int norm, double max_norm, double eps, int out_dtype, void* norm_out, const void* workspace,
-                   int64_t workspace_bytes, void* stream) {
-  return guarded("dla_norm_scale", [&] {
-    return norm_scale_impl(n_tensors, dtypes, tensors, outs, numels, norm, max_norm, eps, out_dtype, norm_out, workspace,
-                           workspace_bytes, stream);
+int dla_norm_clip(int n_tensors, const int* dtypes, const void* const* tensors, void* const* outs, const int64_t* numels,
+                  int norm, double max_norm, double eps, int out_dtype, void* norm_out, void* counter, void* workspace,
+                  int64_t workspace_bytes, void* stream) {
+  return guarded("dla_norm_clip", [&] {
+    return norm_clip_impl(n_tensors, dtypes, tensors, outs, numels, norm, max_norm, eps, out_dtype, norm_out, counter,
+                          workspace, workspace_bytes, stream);
   });
 }
 
@@ -1028,34 +1241,42 @@ int64_t dla_peer_workspace(int n_tensors, int n_peers) {
   return peer_workspace_bytes(n_tensors, n_peers);
 }
 
+int64_t dla_peer_table(int n_tensors, int n_peers) {
+  if (n_tensors < 0 || n_peers < 1 || n_peers > kMostPeers) return 0;
+  const int64_t words = peer_table_words(n_tensors, n_peers);
+  return words <= kPutWords ? 0 : words * 8;
+}
+
 int dla_peer_norms(int n_tensors, const int* dtypes, const void* const* peer_ptrs, const void* const* centers,
-                   const int64_t* numels, int n_peers, double* sq_out, int out_dtype, void* norms, void* workspace,
-                   int64_t workspace_bytes, void* stream) {
+                   const int64_t* numels, int n_peers, double* sq_out, int out_dtype, void* norms, void* counters,
+                   void* table_host, int64_t table_host_bytes, void* workspace, int64_t workspace_bytes, void* stream) {
   return guarded("dla_peer_norms", [&] {
     const Round r = {n_tensors, dtypes, peer_ptrs, centers, nullptr, numels, nullptr, n_peers, {0, 0, 0}, false};
-    return round_impl("dla_peer_norms", r, 0, nullptr, sq_out, out_dtype, norms, workspace, workspace_bytes, stream);
+    return round_impl("dla_peer_norms", r, 0, nullptr, sq_out, out_dtype, norms, counters, table_host, table_host_bytes, workspace, workspace_bytes, stream);
   });
 }
 
 int dla_wsum_bounded(int n_tensors, const int* dtypes, const void* const* peer_ptrs, const void* const* centers,
                      void* const* outs, const int64_t* numels, const double* weights, int n_peers, double max_norm,
-                     const double* sq, int out_dtype, void* norms, void* workspace, int64_t workspace_bytes, void* stream) {
+                     const double* sq, int out_dtype, void* norms, void* counters, void* table_host,
+                     int64_t table_host_bytes, void* workspace, int64_t workspace_bytes, void* stream) {
   return guarded("dla_wsum_bounded", [&] {
     if (!outs && n_tensors > 0) return fail(DLA_E_INVALID, "dla_wsum_bounded: null outs array");
     static void* const none[1] = {nullptr};
     const Round r = {n_tensors, dtypes, peer_ptrs, centers, outs ? outs : none, numels, weights, n_peers, {0, 0, 0}, false};
-    return round_impl("dla_wsum_bounded", r, max_norm, sq, nullptr, out_dtype, norms, workspace, workspace_bytes, stream);
+    return round_impl("dla_wsum_bounded", r, max_norm, sq, nullptr, out_dtype, norms, counters, table_host, table_host_bytes, workspace, workspace_bytes, stream);
   });
 }
 
 int dla_wsum_bounded_slab_tiled(int dtype, const void* base, int64_t tile_elems, int64_t slab_rows, const void* center,
                                 const double* weights, int n_peers, int64_t n_elems, double max_norm, void* out,
-                                int out_dtype, void* norms, void* workspace, int64_t workspace_bytes, void* stream) {
+                                int out_dtype, void* norms, void* counters, void* workspace, int64_t workspace_bytes,
+                                void* stream) {
   return guarded("dla_wsum_bounded_slab_tiled", [&] {
     if (!out && n_elems > 0) return fail(DLA_E_INVALID, "dla_wsum_bounded_slab_tiled: null out");
     SlabRound sr;
     if (int rc = slab_round("dla_wsum_bounded_slab_tiled", &sr, dtype, base, tile_elems, slab_rows, center, n_peers, n_elems, out, weights)) return rc;
-    return round_impl("dla_wsum_bounded_slab_tiled", sr.r, max_norm, nullptr, nullptr, out_dtype, norms, workspace, workspace_bytes, stream);
+    return round_impl("dla_wsum_bounded_slab_tiled", sr.r, max_norm, nullptr, nullptr, out_dtype, norms, counters, nullptr, 0, workspace, workspace_bytes, stream);
   });
 }
 

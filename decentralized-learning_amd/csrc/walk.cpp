@@ -239,11 +239,23 @@ py::object fingerprint(py::object model, py::object plain) {
 // tensors of a norm, its outputs, the peers of a round), from L equally long lists of tensors, or None when
 // some tensor is not what the kernels take as it is — a dense tensor (any order of its axes, nothing skipped
 // or shared) of a supported dtype on one HIP device, with the dtype, sizes and element order of its place in
-// lists[0] — and the caller's own pass says which or copies it.  The tables are
-//     (device index, int32 dtype codes [T], int64 numels [T], uint64 addresses [lead][T] of the first `lead`
-//      lists, uint64 addresses [T][L - lead] of the others, whether any tensor is float64)
-// The tensors of lists[bump] (-1: none) are about to be written: their version counters move on, as torch's
-// own in-place operators do it.  One pass, ~20 ns a tensor (in Python ~1 us, 110 tensors of a ResNet-34).
+// lists[0] — and the caller's own pass says which or copies it.  The tensors of lists[bump] (-1: none) are about to
+// be written: their version counters move on, as torch's own in-place operators do it.  One pass, ~20 ns a
+// tensor (in Python ~1 us, 110 tensors of a ResNet-34).
+struct DenseTables {
+  py::ssize_t n = 0;           // tensors
+  int device = -1;
+  bool wide = false;           // a float64 tensor among them
+  std::vector<int32_t> codes;  // [n] DLA_*
+  std::vector<int64_t> numels;
+  std::vector<uint64_t> head;  // addresses [lead][n] of the first `lead` lists
+  std::vector<uint64_t> tail;  // addresses [n][L - lead] of the others
+  uint64_t codes_at() const { return reinterpret_cast<uint64_t>(codes.data()); }
+  uint64_t numels_at() const { return reinterpret_cast<uint64_t>(numels.data()); }
+  uint64_t lead_at(py::ssize_t i) const { return reinterpret_cast<uint64_t>(head.data() + i * n); }
+  uint64_t rest_at() const { return reinterpret_cast<uint64_t>(tail.data()); }
+};
+
 py::object dense_lists(py::list lists, py::ssize_t lead, py::ssize_t bump) {
   const py::ssize_t n_lists = PyList_GET_SIZE(lists.ptr());
   if (n_lists < 1 || lead < 1 || lead > n_lists) return py::none();
@@ -251,11 +263,17 @@ py::object dense_lists(py::list lists, py::ssize_t lead, py::ssize_t bump) {
   if (!PyList_Check(first)) return py::none();
   const py::ssize_t n = PyList_GET_SIZE(first), rest = n_lists - lead;
   if (n < 1) return py::none();
-  std::vector<int32_t> codes(n);
-  std::vector<int64_t> numels(n);
-  std::vector<uint64_t> head(lead * n), tail(rest * n);
-  int device = -1;
-  bool wide = false;
+  auto tables = std::make_unique<DenseTables>();
+  tables->n = n;
+  tables->codes.resize(n);
+  tables->numels.resize(n);
+  tables->head.resize(lead * n);
+  tables->tail.resize(rest * n);
+  auto &codes = tables->codes;
+  auto &numels = tables->numels;
+  auto &head = tables->head, &tail = tables->tail;
+  int& device = tables->device;
+  bool& wide = tables->wide;
   for (py::ssize_t l = 0; l < n_lists; ++l) {
     PyObject* list = PyList_GET_ITEM(lists.ptr(), l);
     if (!PyList_Check(list) || PyList_GET_SIZE(list) != n) return py::none();
@@ -300,10 +318,7 @@ py::object dense_lists(py::list lists, py::ssize_t lead, py::ssize_t bump) {
       if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
     }
   }
-  auto table = [](const auto& v) {
-    return py::bytearray(reinterpret_cast<const char*>(v.data()), v.size() * sizeof(v[0]));
-  };
-  return py::make_tuple(device, table(codes), table(numels), table(head), table(tail), wide);
+  return py::cast(std::move(tables));
 }
 
 // (addresses, byte lengths) of a list of byte blocks as two int64 arrays — the block list an EVA transfer
@@ -1636,6 +1651,14 @@ PYBIND11_MODULE(_dla_walk, m) {
   m.def("layout", &layout, py::arg("models"), py::arg("device"), py::arg("plain"), py::arg("tensor_major"),
         py::arg("ref") = py::none());
   m.def("tensors", &tensors, py::arg("model"), py::arg("plain"));
+  py::class_<DenseTables>(m, "DenseTables")
+      .def_readonly("n", &DenseTables::n)
+      .def_readonly("device", &DenseTables::device)
+      .def_readonly("wide", &DenseTables::wide)
+      .def_property_readonly("codes", &DenseTables::codes_at)
+      .def_property_readonly("numels", &DenseTables::numels_at)
+      .def_property_readonly("rest", &DenseTables::rest_at)
+      .def("lead", &DenseTables::lead_at);
   m.def("dense_lists", &dense_lists, py::arg("lists"), py::arg("lead"), py::arg("bump"));
   m.def("block_table", &block_table, py::arg("blocks"));
   m.def("fingerprint", &fingerprint, py::arg("model"), py::arg("plain"));

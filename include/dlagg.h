@@ -228,37 +228,44 @@ int dla_mean(int dtype, const void* const* peers, int n_peers, int64_t n_elems, 
  *
  * Tensors are dense and of any of the four dtypes, mixed freely within a call; their pointers need element
  * alignment only.  Sums and norms are carried in 64 bits.  Nothing synchronises; the stream's device must be
- * current.  Launches take everything by value except the caller's buffers, so a captured call replays.  The
- * workspaces are the caller's, need no initialisation and hold nothing between calls (dla_norm's partial sums
- * until the dla_norm_scale behind it has run); two calls in flight at once need two. */
+ * current.  Without a table_host, launches take everything by value except the caller's buffers, so a captured call
+ * replays.  The workspaces are the caller's, need no initialisation and hold nothing between calls; two calls in
+ * flight at once need two.  The counters (NULL: one launch more) let a kernel's last workgroup add up what the others
+ * found: DEVICE memory, DLA_COUNTER_BYTES zero bytes, which are zero again when the call's work is done; calls on one
+ * stream may share them, calls on two must not. */
+#define DLA_COUNTER_BYTES 65536
 #define DLA_NORM_INF 0
 #define DLA_NORM_L1 1
 #define DLA_NORM_L2 2
 
-/* Bytes of the workspace of dla_norm / dla_norm_scale over n_tensors tensors. */
+/* Bytes of the workspace of dla_norm / dla_norm_clip over n_tensors tensors. */
 int64_t dla_norm_workspace(int n_tensors);
 
 /* The norm of all elements of n_tensors tensors together: sqrt(sum x^2), sum |x| or max |x| (0 for no elements;
  * a NaN anywhere gives NaN), what a training step needs before it clips a model's gradient (the reference
  * trains at accdfl/core/model_trainer.py:18-121 and does not clip).
  *   dtypes, tensors, numels  host arrays of n_tensors
- *   out        DEVICE pointer to one value of out_dtype (F32 or F64), or NULL: the partial sums only, for
- *              dla_norm_scale
+ *   out        DEVICE pointer to one value of out_dtype (F32 or F64)
  *   workspace  DEVICE memory of dla_norm_workspace(n_tensors) bytes, 8-byte aligned */
 int dla_norm(int n_tensors, const int* dtypes, const void* const* tensors, const int64_t* numels, int norm, int out_dtype,
-             void* out, void* workspace, int64_t workspace_bytes, void* stream);
+             void* out, void* counter, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* outs[t] = round(tensors[t] * min(1, max_norm / (n + eps))), n the norm whose partial sums dla_norm left in
- * `workspace` for the same tensors, counts and norm earlier on this stream.  NaN norms make everything NaN,
+/* outs[t] = round(tensors[t] * min(1, max_norm / (n + eps))), n the norm of the tensors.  NaN norms make everything NaN,
  * infinite ones give a factor of 0.  outs[t] may be tensors[t]; every other overlap is refused (DLA_E_ALIAS).  In
  * place nothing is written when the factor is 1.  norm_out (F32 or F64, DEVICE) may be NULL. */
-int dla_norm_scale(int n_tensors, const int* dtypes, const void* const* tensors, void* const* outs, const int64_t* numels,
-                   int norm, double max_norm, double eps, int out_dtype, void* norm_out, const void* workspace,
-                   int64_t workspace_bytes, void* stream);
+int dla_norm_clip(int n_tensors, const int* dtypes, const void* const* tensors, void* const* outs, const int64_t* numels,
+                  int norm, double max_norm, double eps, int out_dtype, void* norm_out, void* counter, void* workspace,
+                  int64_t workspace_bytes, void* stream);
 
 /* Bytes of the workspace of dla_peer_norms / dla_wsum_bounded(_slab_tiled, one tensor); 0 for arguments out of
  * range (1 <= n_peers <= 2048). */
 int64_t dla_peer_workspace(int n_tensors, int n_peers);
+
+/* Bytes of page-locked memory that make a call's table travel faster (0: it needs none, up to 480 words of table —
+ * 5 per tensor, one per tensor of a peer, one per peer — go with the launches): table_host below, device-mapped
+ * (hipHostMalloc, torch pin_memory), untouched until the stream has passed the call and so not for captured ones.
+ * NULL is always accepted. */
+int64_t dla_peer_table(int n_tensors, int n_peers);
 
 /* How far each of n_peers models lies from a centre: norms[k] = || p_k - c ||_2 over all tensors together.
  *   peer_ptrs  host array [n_tensors * n_peers] of DEVICE pointers, tensor-major as dla_wsum_multi takes them
@@ -266,8 +273,8 @@ int64_t dla_peer_workspace(int n_tensors, int n_peers);
  *   sq_out     DEVICE doubles [n_peers], the squares (what ranks that hold one bucket each add up), or NULL
  *   norms      DEVICE [n_peers] of out_dtype (F32 or F64), or NULL */
 int dla_peer_norms(int n_tensors, const int* dtypes, const void* const* peer_ptrs, const void* const* centers,
-                   const int64_t* numels, int n_peers, double* sq_out, int out_dtype, void* norms, void* workspace,
-                   int64_t workspace_bytes, void* stream);
+                   const int64_t* numels, int n_peers, double* sq_out, int out_dtype, void* norms, void* counters,
+                   void* table_host, int64_t table_host_bytes, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* fedavg.py:20-25 with every peer's update bounded first:
  *     out = round(c + sum_k a_k (p_k - c)),   a_k = weights[k] * (n_k <= max_norm ? 1 : max_norm / n_k)
@@ -278,13 +285,15 @@ int dla_peer_norms(int n_tensors, const int* dtypes, const void* const* peer_ptr
  *       NULL: computed here */
 int dla_wsum_bounded(int n_tensors, const int* dtypes, const void* const* peer_ptrs, const void* const* centers,
                      void* const* outs, const int64_t* numels, const double* weights, int n_peers, double max_norm,
-                     const double* sq, int out_dtype, void* norms, void* workspace, int64_t workspace_bytes, void* stream);
+                     const double* sq, int out_dtype, void* norms, void* counters, void* table_host,
+                     int64_t table_host_bytes, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* dla_wsum_bounded over rows 0..n_peers-1 of a tile-interleaved slab (the layout of dla_wsum_slab_tiled; any
  * dtype) into the contiguous `out`.  center: a contiguous DEVICE vector (out may be it), or NULL: row 0. */
 int dla_wsum_bounded_slab_tiled(int dtype, const void* base, int64_t tile_elems, int64_t slab_rows, const void* center,
                                 const double* weights, int n_peers, int64_t n_elems, double max_norm, void* out,
-                                int out_dtype, void* norms, void* workspace, int64_t workspace_bytes, void* stream);
+                                int out_dtype, void* norms, void* counters, void* workspace, int64_t workspace_bytes,
+                                void* stream);
 
 /* Largest peer count one kernel pass takes (kernel-argument pointer table). */
 int dla_max_peers_per_pass(void);

@@ -757,6 +757,42 @@ def test_two_captured_graphs_replay_beside_eager_calls():
             no.assert_close(o, w, n, ad)
 
 
+def test_counters_are_zero_again_and_calls_without_them_agree():
+    """Eager calls join in their last workgroup, captured ones in a launch of their own: the same bits."""
+    from accdfl_amd.core import norms
+
+    grads = _list([1 + i * 131 % 9000 for i in range(400)], "bf16", 0.5, seed=21)
+    rounds = [_round(n, [70_003, 5], "f32", seed=n) for n in (1, 8, 9, 130)]
+
+    def everything():
+        out = [norms.global_norm(grads, p) for p in (2.0, 1.0, INF)]
+        clipped, n = norms.clip_global_norm(grads, 0.5)
+        out += clipped + [n]
+        for center, models, weights in rounds:
+            outs = [torch.empty_like(c) for c in center]
+            out += [norms.update_norms(models, center), norms.wsum_bounded_multi(models, weights, center, 3.0, outs)] + outs
+        return out
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        eager = [everything() for _ in range(3)]
+    side.synchronize()
+    for again in eager[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(eager[0], again))
+    assert (0, side.cuda_stream) in norms._counters
+    assert all(int(c.abs().max()) == 0 for c in norms._counters.values())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        captured = everything()
+    for _ in range(3):
+        for t in captured:
+            t.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(eager[0], captured))
+
+
 def test_error_if_nonfinite_is_refused_under_capture():
     from accdfl_amd.core.norms import clip_global_norm_
 

@@ -46,9 +46,9 @@ def _ptrs(*v):
 A, B, WS, BIG = 0x10000, 0x20000, 0x900000, 1 << 30
 
 
-def _norm(L, n=1, codes=None, ptrs=None, numels=None, norm=2, out_code=0, out=0x40000, ws=WS, nbytes=BIG):
-    return _err(L, L.so.dla_norm(n, codes or _ints(0), ptrs or _ptrs(A), numels or _longs(4), norm, out_code, out, ws,
-                                 nbytes, None))
+def _norm(L, n=1, codes=None, ptrs=None, numels=None, norm=2, out_code=0, out=0x40000, counter=None, ws=WS, nbytes=BIG):
+    return _err(L, L.so.dla_norm(n, codes or _ints(0), ptrs or _ptrs(A), numels or _longs(4), norm, out_code, out, counter,
+                                 ws, nbytes, None))
 
 
 @pytest.mark.parametrize("kw, text", [
@@ -62,6 +62,8 @@ def _norm(L, n=1, codes=None, ptrs=None, numels=None, norm=2, out_code=0, out=0x
     (dict(norm=3), "unknown norm"),
     (dict(out_code=1), "F32 or F64"),
     (dict(out_code=3, out=0x40004), "F32 or F64"),
+    (dict(out=None), "null out"),
+    (dict(counter=0x50002), "counter"),
     (dict(ws=None), "workspace"),
     (dict(ws=WS + 4), "workspace"),
     (dict(nbytes=64), "workspace"),
@@ -71,9 +73,10 @@ def test_norm_refusals(L, kw, text):
     assert rc == -1 and text in msg, (rc, msg)
 
 
-def _scale(L, n=1, codes=None, ptrs=None, outs=None, numels=None, max_norm=1.0, eps=1e-6, norm_out=None, ws=WS, nbytes=BIG):
-    return _err(L, L.so.dla_norm_scale(n, codes or _ints(0), ptrs or _ptrs(A), outs or _ptrs(B), numels or _longs(4), 2,
-                                       max_norm, eps, 0, norm_out, ws, nbytes, None))
+def _clip(L, n=1, codes=None, ptrs=None, outs=None, numels=None, max_norm=1.0, eps=1e-6, norm_out=None, counter=None,
+          ws=WS, nbytes=BIG):
+    return _err(L, L.so.dla_norm_clip(n, codes or _ints(0), ptrs or _ptrs(A), outs or _ptrs(B), numels or _longs(4), 2,
+                                      max_norm, eps, 0, norm_out, counter, ws, nbytes, None))
 
 
 @pytest.mark.parametrize("kw, rc_want, text", [
@@ -82,7 +85,8 @@ def _scale(L, n=1, codes=None, ptrs=None, outs=None, numels=None, max_norm=1.0, 
     (dict(eps=-1.0), -1, "eps"),
     (dict(outs=_ptrs(None)), -1, "null"),
     (dict(outs=_ptrs(B + 1)), -1, "not aligned"),
-    (dict(norm_out=0x40002), -1, "norm_out"),
+    (dict(norm_out=0x40002), -1, "F32 or F64"),
+    (dict(counter=0x50001), -1, "counter"),
     (dict(ws=None), -1, "workspace"),
     # an output a part of its own input, of another input, of another output; the same tensor twice
     (dict(outs=_ptrs(A + 4)), -2, "overlaps"),
@@ -91,17 +95,17 @@ def _scale(L, n=1, codes=None, ptrs=None, outs=None, numels=None, max_norm=1.0, 
     (dict(n=2, codes=_ints(0, 0), ptrs=_ptrs(A, A), outs=_ptrs(A, A), numels=_longs(4, 4)), -2, "overlap"),
     (dict(n=2, codes=_ints(0, 0), ptrs=_ptrs(A, A + 8), outs=_ptrs(A, A + 8), numels=_longs(4, 4)), -2, "overlap"),
 ])
-def test_norm_scale_refusals(L, kw, rc_want, text):
-    rc, msg = _scale(L, **kw)
+def test_norm_clip_refusals(L, kw, rc_want, text):
+    rc, msg = _clip(L, **kw)
     assert rc == rc_want and text in msg, (rc, msg)
 
 
 def _bounded(L, n=1, peers=2, codes=None, ptrs=None, centers=None, outs=None, numels=None, weights=True, max_norm=1.0,
-             norms=None, ws=WS, nbytes=BIG):
+             norms=None, counters=None, ws=WS, nbytes=BIG):
     return _err(L, L.so.dla_wsum_bounded(
         n, codes or _ints(0), ptrs or _ptrs(A, B), centers or _ptrs(0x30000), outs or _ptrs(0x40000), numels or _longs(4),
-        (ctypes.c_double * max(1, peers))(*[0.5] * max(1, peers)) if weights else None, peers, max_norm, None, 0, norms, ws,
-        nbytes, None))
+        (ctypes.c_double * max(1, peers))(*[0.5] * max(1, peers)) if weights else None, peers, max_norm, None, 0, norms, counters,
+        None, 0, ws, nbytes, None))
 
 
 @pytest.mark.parametrize("kw, rc_want, text", [
@@ -118,6 +122,7 @@ def _bounded(L, n=1, peers=2, codes=None, ptrs=None, centers=None, outs=None, nu
     (dict(max_norm=-0.5), -1, "max_norm"),
     (dict(max_norm=math.nan), -1, "max_norm"),
     (dict(norms=0x50002), -1, "norms"),
+    (dict(counters=0x50002), -1, "counters"),
     (dict(ws=None), -1, "workspace"),
     (dict(nbytes=128), -1, "workspace"),
     (dict(outs=_ptrs(B + 4)), -2, "peer 1"),
@@ -152,7 +157,7 @@ def test_bounded_slab_refusals(L, kw, rc_want, text):
     a.update(kw)
     rc = L.so.dla_wsum_bounded_slab_tiled(a["dtype"], a["base"], a["tile"], a["rows"], a["center"],
                                           (ctypes.c_double * 2)(0.5, 0.5), a["n"], a["numel"], a["max_norm"], a["out"], 0,
-                                          None, WS, BIG, None)
+                                          None, None, WS, BIG, None)
     rc, msg = _err(L, rc)
     assert rc == rc_want and text in msg, (rc, msg)
 
