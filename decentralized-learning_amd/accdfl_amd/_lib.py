@@ -491,59 +491,31 @@ def mean_ptrs(dtype_code: int, peer_ptrs: Sequence[int], n_elems: int, out_ptr: 
 NORM_CODES = {2.0: 2, 1.0: 1, float("inf"): 0}  # DLA_NORM_*
 COUNTER_BYTES = 65536  # DLA_COUNTER_BYTES
 
-# The norm entry points take their tables (dtype codes, device pointers, counts) as addresses.
+
+_entry: dict = {}
+
+
+def entry(name: str) -> int:
+    """The address of an entry point (the walk extension calls the norm entry points by it)."""
+    a = _entry.get(name)
+    if a is None:
+        a = _entry[name] = ctypes.cast(getattr(lib().so, name), ctypes.c_void_p).value
+    return a
 
 
 def norm_workspace(n_tensors: int) -> int:
-    """dla_norm_workspace: bytes of the workspace of norm_ptrs / norm_clip_ptrs."""
+    """dla_norm_workspace: bytes of the workspace of dla_norm / dla_norm_clip."""
     return lib().so.dla_norm_workspace(n_tensors)
 
 
-def norm_ptrs(*args) -> None:
-    """dla_norm(n_tensors, dtypes, tensors, numels, norm, out_dtype, out, counter, workspace, bytes, stream)."""
-    L = lib()
-    rc = L.so.dla_norm(*args)
-    if rc:
-        L.check(rc, "dla_norm")
-
-
-def norm_clip_ptrs(*args) -> None:
-    """dla_norm_clip(n_tensors, dtypes, tensors, outs, numels, norm, max_norm, eps, out_dtype, norm_out, counter,
-    workspace, bytes, stream)."""
-    L = lib()
-    rc = L.so.dla_norm_clip(*args)
-    if rc:
-        L.check(rc, "dla_norm_clip")
-
-
 def peer_workspace(n_tensors: int, n_peers: int) -> int:
-    """dla_peer_workspace: bytes of the workspace of peer_norms_ptrs / wsum_bounded_ptrs (0: out of range)."""
+    """dla_peer_workspace: bytes of the workspace of dla_peer_norms / dla_wsum_bounded (0: out of range)."""
     return lib().so.dla_peer_workspace(n_tensors, n_peers)
 
 
 def peer_table(n_tensors: int, n_peers: int) -> int:
     """dla_peer_table: bytes of page-locked memory a call of this size is faster with (0: none)."""
     return lib().so.dla_peer_table(n_tensors, n_peers)
-
-
-def peer_norms_ptrs(*args) -> None:
-    """dla_peer_norms(n_tensors, dtypes, peers, centers, numels, n_peers, sq, out_dtype, norms, counters, table_host,
-    table_bytes, workspace, bytes, stream)."""
-    L = lib()
-    rc = L.so.dla_peer_norms(*args)
-    if rc:
-        L.check(rc, "dla_peer_norms")
-
-
-def wsum_bounded_ptrs(n_tensors: int, codes, peers, centers, outs, numels, weights: Sequence[float], n_peers: int,
-                      *args) -> None:
-    """dla_wsum_bounded(n_tensors, dtypes, peers, centers, outs, numels, weights, n_peers, max_norm, sq, out_dtype,
-    norms, counters, table_host, table_bytes, workspace, bytes, stream)."""
-    L = lib()
-    _check_tables("wsum_bounded", n_peers, 1, weights=weights)
-    rc = L.so.dla_wsum_bounded(n_tensors, codes, peers, centers, outs, numels, _dbl_array(weights), n_peers, *args)
-    if rc:
-        L.check(rc, "dla_wsum_bounded")
 
 
 def wsum_bounded_slab_tiled_ptr(dtype_code: int, base_ptr: int, tile_elems: int, slab_rows: int, center_ptr,

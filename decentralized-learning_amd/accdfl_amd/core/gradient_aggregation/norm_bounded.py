@@ -18,7 +18,6 @@ and the centre must have the same parameters (count, shapes, dtypes).
 """
 from __future__ import annotations
 
-import ctypes
 from typing import List, Optional
 
 import torch
@@ -36,23 +35,25 @@ def _device_round(models: List[nn.Module], weights, center: nn.Module, max_norm:
     result's parameters made around the launches as FedAvg's device round makes them.  None when the models do
     not qualify (the general path then handles the round)."""
     mod = _lib.walk_module()
-    layout = _fedavg._device_layout([center] + models) if mod is not None and hasattr(mod, "param_blocks") else None
-    if layout is None:
+    if mod is None:
         return None
-    dtype, device, numels, table = layout
+    everything = [center] + models
+    tables = mod.module_tables(everything, _fedavg._PLAIN_SET)
+    if tables is None:
+        # classes not met before are classified once, as FedAvg's layout does it
+        fresh = {type(sub) for m in (center, models[0]) for sub in m.modules()} - _fedavg._plain_walk_cls.keys()
+        if any([_fedavg._plain_walk(cls) for cls in fresh]):
+            tables = mod.module_tables(everything, _fedavg._PLAIN_SET)
+    if tables is None:
+        return None
     objs = mod.tensors(models[0], _fedavg._PLAIN_SET)
-    if objs is None or len(objs[0]) != len(numels) or any(type(p) is not nn.Parameter for p in objs[0]):
+    if objs is None or any([type(p) is not nn.Parameter for p in objs[0]]):
         return None
     p0, b0 = objs
-    n, t = len(models), len(numels)
     memo = {}
-    with _norms._place(device, None):
-        blocks, out_ptrs = mod.param_blocks(p0)
-        address = ctypes.c_void_p * t
-        tables = _norms._Tables(device.index, dtype == torch.float64, (ctypes.c_int * t)(*[_wsum.dtype_code(dtype)] * t),
-                                _fedavg._flat_plan(dtype, numels)[3], [address.from_buffer(table[:, 0].copy())],
-                                (ctypes.c_void_p * (t * n)).from_buffer(table[:, 1:].copy()))
-        _norms.wsum_bounded_tables(tables, out_ptrs.ctypes.data, weights, n, max_norm)
+    with _norms._place(torch.device("cuda", tables.device), None):
+        blocks, outs = mod.param_blocks(p0)
+        _norms.wsum_bounded_tables(tables, outs, weights, max_norm)
         # while the round runs: the parameters' Python objects, models[0]'s buffers, the module tree
         mod.param_wrap(blocks, p0, memo)
         _fedavg._seed_buffers(b0, memo)
@@ -113,7 +114,7 @@ class NormBoundedFedAvg(GradientAggregation):
             weights = [float(1. / len(models)) for _ in range(len(models))]
         else:
             assert len(weights) == len(models)
-        weights = list(weights)
+        weights = [float(w) for w in weights]
         models = list(models)
         _norms._check_peers(len(models))
         with torch.no_grad():

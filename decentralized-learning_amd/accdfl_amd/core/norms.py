@@ -41,23 +41,48 @@ MAX_PEERS = 2048  # include/dlagg.h dla_peer_workspace
 
 # ------------------------------------------------------------------------------------------- tables of tensors
 class _Tables:
-    """What one call hands to the library, with the attributes of the walk extension's DenseTables: ``n`` tensors on
-    HIP device ``device``, ``wide``: float64 among them, and the addresses of the tables — dtype codes, counts, the
-    i-th of the first lists, the other lists tensor-major.  ``keep``: what owns them."""
+    """The walk extension's DenseTables (csrc/walk.cpp: what a call hands to the library, and the calls) in Python,
+    for when the extension is absent: ``n`` tensors on HIP device ``device``; dtype codes, counts, the addresses of
+    the first lists, and those of the other lists tensor-major."""
 
-    __slots__ = ("n", "device", "wide", "codes", "numels", "leads", "rest", "keep")
-
-    def __init__(self, device: int, wide: bool, codes, numels, leads, rest):
-        self.n = len(codes)
+    def __init__(self, device: int, lists: List[List[torch.Tensor]], lead: int):
+        n, rest = len(lists[0]), lists[lead:]
+        address = lambda t: t.data_ptr() if t.numel() else 0  # noqa: E731
+        self.n = n
         self.device = device
-        self.wide = wide
-        self.keep = (codes, numels, leads, rest)
-        self.codes, self.numels = ctypes.addressof(codes), ctypes.addressof(numels)
-        self.leads = [ctypes.addressof(x) for x in leads]
-        self.rest = None if rest is None else ctypes.addressof(rest)
+        self.wide = any(t.dtype == torch.float64 for t in lists[0])
+        self.codes = (ctypes.c_int * n)(*[_wsum.dtype_code(t.dtype) for t in lists[0]])
+        self.numels = (ctypes.c_int64 * n)(*[t.numel() for t in lists[0]])
+        self.lead = [(ctypes.c_void_p * n)(*[address(t) for t in ts]) for ts in lists[:lead]]
+        self.rest = (ctypes.c_void_p * (n * len(rest)))(*[address(ts[i]) for i in range(n) for ts in rest])
 
-    def lead(self, i: int) -> int:
-        return self.leads[i]
+    def _result(self, size, double: bool):
+        return torch.empty(size, dtype=torch.float64 if double else torch.float32, device=self.device)
+
+    def _call(self, name: str, out, *args):
+        return getattr(_lib.lib().so, name)(self.n, self.codes, *args), out
+
+    def norm(self, fn, code, counter, nbytes, stream):
+        out, ws = self._result((), self.wide), _workspace(nbytes, self.device)
+        return self._call("dla_norm", out, self.lead[0], self.numels, code, 3 * self.wide, out.data_ptr(), counter,
+                          ws.data_ptr(), nbytes, stream)
+
+    def clip(self, fn, code, max_norm, eps, counter, nbytes, stream):
+        out, ws = self._result((), self.wide), _workspace(nbytes, self.device)
+        return self._call("dla_norm_clip", out, self.lead[0], self.lead[1], self.numels, code, max_norm, eps,
+                          3 * self.wide, out.data_ptr(), counter, ws.data_ptr(), nbytes, stream)
+
+    def peer_norms(self, fn, n, squared, counters, table, table_bytes, nbytes, stream):
+        out, ws = self._result(n, squared or self.wide), _workspace(nbytes, self.device)
+        return self._call("dla_peer_norms", out, self.rest, self.lead[0], self.numels, n, out.data_ptr() if squared else 0,
+                          3 * self.wide, 0 if squared else out.data_ptr(), counters, table, table_bytes, ws.data_ptr(),
+                          nbytes, stream)
+
+    def bounded(self, fn, outs, weights, max_norm, sq, counters, table, table_bytes, nbytes, stream):
+        out, ws = self._result(len(weights), self.wide), _workspace(nbytes, self.device)
+        return self._call("dla_wsum_bounded", out, self.rest, self.lead[0], self.lead[1], self.numels,
+                          _lib._dbl_array(weights), len(weights), max_norm, sq, 3 * self.wide, out.data_ptr(), counters,
+                          table, table_bytes, ws.data_ptr(), nbytes, stream)
 
 
 def _pack(lists: List[List[torch.Tensor]], lead: int, bump: int = -1):
@@ -130,17 +155,16 @@ def _pack_checked(lists: List[List[torch.Tensor]], names: Sequence[str], lead: i
                 back.append((place[out], lists[out][i]))
     tables = _pack(lists, lead, out)
     if tables is None:
-        n, rest = len(lists[0]), lists[lead:]
-        row = ctypes.c_void_p * n
-        address = lambda t: t.data_ptr() if t.numel() else 0  # noqa: E731
-        tables = _Tables(device.index, any(t.dtype == torch.float64 for t in lists[0]), (ctypes.c_int * n)(*[_wsum.dtype_code(t.dtype) for t in lists[0]]),
-                         (ctypes.c_int64 * n)(*[t.numel() for t in lists[0]]),
-                         [row(*[address(t) for t in ts]) for ts in lists[:lead]],
-                         (ctypes.c_void_p * (n * len(rest)))(*[address(ts[i]) for i in range(n) for ts in rest])
-                         if rest else None)
+        tables = _Tables(device.index, lists, lead)
         if out >= 0:
             torch.autograd.graph.increment_version([t for t in lists[out] if not t.is_inference()])
     return tables, back, lists  # the lists keep the copies alive until the call is enqueued
+
+
+def _write_back(pairs) -> None:
+    with torch.no_grad():
+        for t, copy in pairs:
+            t.copy_(copy)
 
 
 def _tensors_of(what: Tensors) -> List[torch.Tensor]:
@@ -198,11 +222,6 @@ def _workspace(nbytes: int, device: int) -> torch.Tensor:
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
-def _result_type(tables):
-    """(torch dtype, DLA_* code) of a call's norms."""
-    return (torch.float64, _lib.DLA_F64) if tables.wide else (torch.float32, _lib.DLA_F32)
-
-
 # Counters of the library's last-workgroup joins (include/dlagg.h): zero before and after every call, so the calls of
 # one stream share one set — (device, stream handle) -> tensor.  A captured call takes none (a replay may run on
 # another stream): it joins in a launch of its own.  Nor does hipStreamPerThread, one handle for many streams.
@@ -210,9 +229,10 @@ _counters: Dict[Tuple[int, int], torch.Tensor] = {}
 _STREAM_PER_THREAD = 2
 
 
-def _counter(device: int, raw_stream: int) -> Optional[int]:
+def _counter(device: int, raw_stream: int) -> int:
+    """The address of the stream's counters, or 0."""
     if raw_stream == _STREAM_PER_THREAD or torch.cuda.is_current_stream_capturing():
-        return None
+        return 0
     t = _counters.get((device, raw_stream))
     if t is None:
         t = _counters.setdefault((device, raw_stream), torch.zeros(_lib.COUNTER_BYTES // 4, dtype=torch.int32,
@@ -247,13 +267,10 @@ def global_norm(tensors: Tensors, norm_type: float = 2.0, error_if_nonfinite: bo
         tables, keep = _pack([tensors], 1), None
         if tables is None:
             tables, _, keep = _pack_checked([tensors], ["tensors"], 1)
-        dtype, out_code = _result_type(tables)
-        out = torch.empty((), dtype=dtype, device=tables.device)
-        nbytes = _lib.norm_workspace(tables.n)
-        ws = _workspace(nbytes, tables.device)
         raw = _raw_stream(tables.device)
-        _lib.norm_ptrs(tables.n, tables.codes, tables.lead(0), tables.numels, code, out_code, out.data_ptr(),
-                       _counter(tables.device, raw), ws.data_ptr(), nbytes, raw)
+        rc, out = tables.norm(_lib.entry("dla_norm"), code, _counter(tables.device, raw), _lib.norm_workspace(tables.n), raw)
+        if rc:
+            _lib.lib().check(rc, "dla_norm")
         del keep
         if error_if_nonfinite:
             _refuse_nonfinite(out, norm_type)
@@ -271,7 +288,7 @@ def clip_global_norm(tensors: Tensors, max_norm: float, norm_type: float = 2.0, 
     code = _norm_code(norm_type)
     bound = _bound(max_norm)
     tensors = _tensors_of(tensors)
-    with _place(_device_of(tensors, stream), stream), torch.no_grad():
+    with _place(_device_of(tensors, stream), stream):
         if error_if_nonfinite:
             _refuse_capture()
         if outs is None:
@@ -285,20 +302,18 @@ def clip_global_norm(tensors: Tensors, max_norm: float, norm_type: float = 2.0, 
         tables, back, keep = _pack([tensors, outs], 2, bump=1), (), None
         if tables is None:
             tables, back, keep = _pack_checked([tensors, outs], ["tensors", "outs"], 2, out=1)
-        dtype, out_code = _result_type(tables)
-        norm = torch.empty((), dtype=dtype, device=tables.device)
-        nbytes = _lib.norm_workspace(tables.n)
-        ws = _workspace(nbytes, tables.device)
         raw = _raw_stream(tables.device)
-        counter = _counter(tables.device, raw)
+        counter, nbytes = _counter(tables.device, raw), _lib.norm_workspace(tables.n)
         if error_if_nonfinite:
-            _lib.norm_ptrs(tables.n, tables.codes, tables.lead(0), tables.numels, code, out_code, norm.data_ptr(),
-                           counter, ws.data_ptr(), nbytes, raw)
+            rc, norm = tables.norm(_lib.entry("dla_norm"), code, counter, nbytes, raw)
+            if rc:
+                _lib.lib().check(rc, "dla_norm")
             _refuse_nonfinite(norm, norm_type)
-        _lib.norm_clip_ptrs(tables.n, tables.codes, tables.lead(0), tables.lead(1), tables.numels, code, bound, CLIP_EPS,
-                            out_code, norm.data_ptr(), counter, ws.data_ptr(), nbytes, raw)
-        for t, copy in back:
-            t.copy_(copy)
+        rc, norm = tables.clip(_lib.entry("dla_norm_clip"), code, bound, CLIP_EPS, counter, nbytes, raw)
+        if rc:
+            _lib.lib().check(rc, "dla_norm_clip")
+        if back:
+            _write_back(back)
         del keep
         return list(outs), norm
 
@@ -334,22 +349,29 @@ def _check_peers(n: int) -> None:
 
 
 @contextlib.contextmanager
-def _table_host(n_tensors: int, n: int, device: int):
-    """(address, bytes) of page-locked memory for a round's table, or (None, 0): the table is small enough to go with
+def _ring_slot(nbytes: int, device: int):
+    """(address, bytes) of page-locked memory for a round's table, or (0, 0): the table is small enough to go with
     the launches, the call is being captured (its launches then carry the table by value), or every slot of the
     device's ring is in use."""
-    nbytes = _lib.peer_table(n_tensors, n)
     slot = None
     if nbytes and not torch.cuda.is_current_stream_capturing():
         ring = _wsum.table_ring(torch.device("cuda", device))
         slot = ring.take(nbytes, wait=False)
     if slot is None:
-        yield None, 0
+        yield 0, 0
         return
     try:
         yield slot[1].data_ptr(), nbytes
     finally:
         ring.done(slot[0], torch.cuda.current_stream(device), fence=True)
+
+
+_NO_TABLE = contextlib.nullcontext((0, 0))
+
+
+def _table_host(n_tensors: int, n: int, device: int):
+    nbytes = _lib.peer_table(n_tensors, n)
+    return _ring_slot(nbytes, device) if nbytes else _NO_TABLE
 
 
 def update_norms(models: Sequence[Tensors], center: Tensors, stream: Optional[torch.cuda.Stream] = None,
@@ -365,32 +387,28 @@ def update_norms(models: Sequence[Tensors], center: Tensors, stream: Optional[to
         if not lists[0] and not any(lists):
             return torch.zeros(n, dtype=torch.float64 if squared else torch.float32, device=device)
         tables, _, keep = _pack_round(lists, lambda: ["center"] + ["model %d" % k for k in range(n)], 1)
-        dtype, out_code = _result_type(tables)
-        out = torch.empty(n, dtype=torch.float64 if squared else dtype, device=tables.device)
-        nbytes = _lib.peer_workspace(tables.n, n)
-        ws = _workspace(nbytes, tables.device)
         raw = _raw_stream(tables.device)
-        with _table_host(tables.n, n, tables.device) as (host, host_bytes):
-            _lib.peer_norms_ptrs(tables.n, tables.codes, tables.rest, tables.lead(0), tables.numels, n,
-                                 out.data_ptr() if squared else None, out_code, None if squared else out.data_ptr(),
-                                 _counter(tables.device, raw), host, host_bytes, ws.data_ptr(), nbytes, raw)
+        with _table_host(tables.n, n, tables.device) as (table, table_bytes):
+            rc, out = tables.peer_norms(_lib.entry("dla_peer_norms"), n, squared, _counter(tables.device, raw), table,
+                                        table_bytes, _lib.peer_workspace(tables.n, n), raw)
+            if rc:
+                _lib.lib().check(rc, "dla_peer_norms")
         del keep
         return out
 
 
-def wsum_bounded_tables(tables, outs: int, weights: Sequence[float], n: int, max_norm: float,
+def wsum_bounded_tables(tables, outs, weights: Sequence[float], max_norm: float,
                         sq_norms: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """dla_wsum_bounded on packed tables (``lead(0)`` the centre, ``rest`` the peers, ``outs`` the address of the
-    outputs' table) on the current stream; returns the update norms [n]."""
-    dtype, out_code = _result_type(tables)
-    norms = torch.empty(n, dtype=dtype, device=tables.device)
-    nbytes = _lib.peer_workspace(tables.n, n)
-    ws = _workspace(nbytes, tables.device)
+    """dla_wsum_bounded on packed tables (the centre first, then the outputs unless ``outs`` has their addresses, then
+    the peers) on the current stream; returns the update norms [n]."""
+    n = len(weights)
     raw = _raw_stream(tables.device)
-    with _table_host(tables.n, n, tables.device) as (host, host_bytes):
-        _lib.wsum_bounded_ptrs(tables.n, tables.codes, tables.rest, tables.lead(0), outs, tables.numels, weights, n,
-                               max_norm, None if sq_norms is None else sq_norms.data_ptr(), out_code, norms.data_ptr(),
-                               _counter(tables.device, raw), host, host_bytes, ws.data_ptr(), nbytes, raw)
+    with _table_host(tables.n, n, tables.device) as (table, table_bytes):
+        rc, norms = tables.bounded(_lib.entry("dla_wsum_bounded"), outs, weights, max_norm,
+                                   0 if sq_norms is None else sq_norms.data_ptr(), _counter(tables.device, raw), table,
+                                   table_bytes, _lib.peer_workspace(tables.n, n), raw)
+        if rc:
+            _lib.lib().check(rc, "dla_wsum_bounded")
     return norms
 
 
@@ -414,16 +432,16 @@ def wsum_bounded_multi(peer_params: Sequence[Tensors], weights: Sequence[float],
     if len(weights) != n:
         raise AssertionError("len(weights) != len(peers)")
     device = _device_of(lists[0], stream)
-    with _place(device, stream), torch.no_grad():
+    with _place(device, stream):
         if not any(lists):
             return torch.zeros(n, dtype=torch.float32, device=device) if sq_norms is None else sq_norms.sqrt().float()
         tables, back, keep = _pack_round(lists, lambda: ["center", "outs"] + ["peer %d" % k for k in range(n)], 2, out=1)
         if sq_norms is not None and (sq_norms.dtype != torch.float64 or sq_norms.numel() != n
                                      or sq_norms.device != device or not sq_norms.is_contiguous()):
             raise ValueError("sq_norms must be %d contiguous float64 values on %s" % (n, device))
-        norms = wsum_bounded_tables(tables, tables.lead(1), weights, n, bound, sq_norms)
-        for t, copy in back:
-            t.copy_(copy)
+        norms = wsum_bounded_tables(tables, None, [float(w) for w in weights], bound, sq_norms)
+        if back:
+            _write_back(back)
         del keep
         return norms
 

@@ -235,13 +235,11 @@ py::object fingerprint(py::object model, py::object plain) {
   return py::bytes(reinterpret_cast<const char*>(v.data()), v.size() * sizeof(uint64_t));
 }
 
-// dense_lists(lists, lead, bump): the tables of an operator over many device tensors (core/norms.py: the
-// tensors of a norm, its outputs, the peers of a round), from L equally long lists of tensors, or None when
-// some tensor is not what the kernels take as it is — a dense tensor (any order of its axes, nothing skipped
-// or shared) of a supported dtype on one HIP device, with the dtype, sizes and element order of its place in
-// lists[0] — and the caller's own pass says which or copies it.  The tensors of lists[bump] (-1: none) are about to
-// be written: their version counters move on, as torch's own in-place operators do it.  One pass, ~20 ns a
-// tensor (in Python ~1 us, 110 tensors of a ResNet-34).
+// The tables of an operator over many device tensors (core/norms.py: the tensors of a norm, its outputs, the peers
+// of a round), and its calls of the library on them — addresses of include/dlagg.h's entry points, which this
+// extension is not linked against — with their result and workspace made here: a call costs one Python frame
+// instead of a dozen (the norm of 14 tensors 10.5 -> 7 us of host time, of which the launch is 3).  The device is
+// current and `stream` its current stream when they are called.
 struct DenseTables {
   py::ssize_t n = 0;           // tensors
   int device = -1;
@@ -250,75 +248,178 @@ struct DenseTables {
   std::vector<int64_t> numels;
   std::vector<uint64_t> head;  // addresses [lead][n] of the first `lead` lists
   std::vector<uint64_t> tail;  // addresses [n][L - lead] of the others
-  uint64_t codes_at() const { return reinterpret_cast<uint64_t>(codes.data()); }
-  uint64_t numels_at() const { return reinterpret_cast<uint64_t>(numels.data()); }
-  uint64_t lead_at(py::ssize_t i) const { return reinterpret_cast<uint64_t>(head.data() + i * n); }
-  uint64_t rest_at() const { return reinterpret_cast<uint64_t>(tail.data()); }
+  const uint64_t* lead(py::ssize_t i) const { return head.data() + i * n; }
+
+  at::Tensor result(at::IntArrayRef sizes, bool doubles) const {
+    return at::empty(sizes, at::TensorOptions().dtype(doubles ? at::kDouble : at::kFloat).device(at::kCUDA, device));
+  }
+  at::Tensor bytes(int64_t n_bytes) const {
+    return at::empty({n_bytes}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device));
+  }
+  static void* ptr(uint64_t a) { return reinterpret_cast<void*>(a); }
+  // The call without the interpreter lock: a launch waits while the device's queue is full.
+  template <class Fn, class... Args>
+  static int unlocked(uint64_t fn, Args... args) {
+    py::gil_scoped_release release;
+    return reinterpret_cast<Fn>(fn)(args...);
+  }
+  int out_code() const { return wide ? 3 : 0; }  // DLA_F64 : DLA_F32
+
+  // dla_norm: (status, the norm)
+  py::tuple norm(uint64_t fn, int norm_code, uint64_t counter, int64_t ws_bytes, uint64_t stream) const {
+    using Fn = int (*)(int, const int*, const void* const*, const int64_t*, int, int, void*, void*, void*, int64_t, void*);
+    const at::Tensor out = result({}, wide), ws = bytes(ws_bytes);
+    const int rc = unlocked<Fn>(fn, static_cast<int>(n), codes.data(), reinterpret_cast<const void* const*>(lead(0)),
+                                            numels.data(), norm_code, out_code(), out.data_ptr(), ptr(counter),
+                                            ws.data_ptr(), ws_bytes, ptr(stream));
+    return py::make_tuple(rc, out);
+  }
+  // dla_norm_clip of the first list into the second: (status, the norm)
+  py::tuple clip(uint64_t fn, int norm_code, double max_norm, double eps, uint64_t counter, int64_t ws_bytes,
+                 uint64_t stream) const {
+    using Fn = int (*)(int, const int*, const void* const*, void* const*, const int64_t*, int, double, double, int, void*,
+                       void*, void*, int64_t, void*);
+    const at::Tensor out = result({}, wide), ws = bytes(ws_bytes);
+    const int rc = unlocked<Fn>(
+        fn, static_cast<int>(n), codes.data(), reinterpret_cast<const void* const*>(lead(0)),
+        reinterpret_cast<void* const*>(const_cast<uint64_t*>(lead(1))), numels.data(), norm_code, max_norm, eps,
+        out_code(), out.data_ptr(), ptr(counter), ws.data_ptr(), ws_bytes, ptr(stream));
+    return py::make_tuple(rc, out);
+  }
+  // dla_peer_norms of the other lists around the first: (status, norms or float64 squares)
+  py::tuple peer_norms(uint64_t fn, int n_peers, bool squared, uint64_t counters, uint64_t table, int64_t table_bytes,
+                       int64_t ws_bytes, uint64_t stream) const {
+    using Fn = int (*)(int, const int*, const void* const*, const void* const*, const int64_t*, int, double*, int, void*,
+                       void*, void*, int64_t, void*, int64_t, void*);
+    const at::Tensor out = result({n_peers}, squared || wide), ws = bytes(ws_bytes);
+    void* o = out.data_ptr();
+    const int rc = unlocked<Fn>(
+        fn, static_cast<int>(n), codes.data(), reinterpret_cast<const void* const*>(tail.data()),
+        reinterpret_cast<const void* const*>(lead(0)), numels.data(), n_peers, squared ? static_cast<double*>(o) : nullptr,
+        out_code(), squared ? nullptr : o, ptr(counters), ptr(table), table_bytes, ws.data_ptr(), ws_bytes, ptr(stream));
+    return py::make_tuple(rc, out);
+  }
+  // dla_wsum_bounded of the other lists around the first, into `outs` (addresses; None: the second list):
+  // (status, the norms)
+  py::tuple bounded(uint64_t fn, py::object outs, const std::vector<double>& weights, double max_norm, uint64_t sq,
+                    uint64_t counters, uint64_t table, int64_t table_bytes, int64_t ws_bytes, uint64_t stream) const {
+    using Fn = int (*)(int, const int*, const void* const*, const void* const*, void* const*, const int64_t*, const double*,
+                       int, double, const double*, int, void*, void*, void*, int64_t, void*, int64_t, void*);
+    const uint64_t* to = nullptr;
+    py::array_t<uint64_t, py::array::c_style> given;
+    if (outs.is_none()) {
+      if (head.size() < 2 * static_cast<size_t>(n)) throw std::invalid_argument("bounded: no outputs");
+      to = lead(1);
+    } else {
+      given = outs.cast<py::array_t<uint64_t, py::array::c_style>>();
+      if (given.size() != n) throw std::invalid_argument("bounded: one output per tensor");
+      to = given.data();
+    }
+    if (tail.size() != weights.size() * static_cast<size_t>(n)) throw std::invalid_argument("bounded: one weight per peer");
+    const int n_peers = static_cast<int>(weights.size());
+    const at::Tensor out = result({n_peers}, wide), ws = bytes(ws_bytes);
+    const int rc = unlocked<Fn>(
+        fn, static_cast<int>(n), codes.data(), reinterpret_cast<const void* const*>(tail.data()),
+        reinterpret_cast<const void* const*>(lead(0)), reinterpret_cast<void* const*>(const_cast<uint64_t*>(to)),
+        numels.data(), weights.data(), n_peers, max_norm, reinterpret_cast<const double*>(sq), out_code(), out.data_ptr(),
+        ptr(counters), ptr(table), table_bytes, ws.data_ptr(), ws_bytes, ptr(stream));
+    return py::make_tuple(rc, out);
+  }
 };
 
-py::object dense_lists(py::list lists, py::ssize_t lead, py::ssize_t bump) {
-  const py::ssize_t n_lists = PyList_GET_SIZE(lists.ptr());
-  if (n_lists < 1 || lead < 1 || lead > n_lists) return py::none();
-  PyObject* first = PyList_GET_ITEM(lists.ptr(), 0);
-  if (!PyList_Check(first)) return py::none();
-  const py::ssize_t n = PyList_GET_SIZE(first), rest = n_lists - lead;
-  if (n < 1) return py::none();
+// The tables of L equally long lists of tensors, or null when some tensor is not what the kernels take as it is — a
+// dense tensor (any order of its axes, nothing skipped or shared) of a supported dtype on one HIP device, with the
+// dtype, sizes and element order of its place in lists[0].  ~20 ns a tensor.
+std::unique_ptr<DenseTables> pack_lists(const std::vector<std::vector<PyObject*>>& lists, size_t lead) {
+  const size_t n = lists[0].size(), rest = lists.size() - lead;
   auto tables = std::make_unique<DenseTables>();
-  tables->n = n;
+  tables->n = static_cast<py::ssize_t>(n);
   tables->codes.resize(n);
   tables->numels.resize(n);
   tables->head.resize(lead * n);
   tables->tail.resize(rest * n);
-  auto &codes = tables->codes;
-  auto &numels = tables->numels;
-  auto &head = tables->head, &tail = tables->tail;
-  int& device = tables->device;
-  bool& wide = tables->wide;
-  for (py::ssize_t l = 0; l < n_lists; ++l) {
-    PyObject* list = PyList_GET_ITEM(lists.ptr(), l);
-    if (!PyList_Check(list) || PyList_GET_SIZE(list) != n) return py::none();
-    for (py::ssize_t t = 0; t < n; ++t) {
-      PyObject* o = PyList_GET_ITEM(list, t);
-      if (!THPVariable_Check(o)) return py::none();
+  int device = -1;
+  for (size_t l = 0; l < lists.size(); ++l) {
+    if (lists[l].size() != n) return nullptr;
+    for (size_t t = 0; t < n; ++t) {
+      PyObject* o = lists[l][t];
+      if (!THPVariable_Check(o)) return nullptr;
       const at::Tensor& x = THPVariable_Unpack(o);
       if (x.layout() != at::kStrided || !x.is_cuda() || x.is_neg() || x.unsafeGetTensorImpl()->is_python_dispatch() ||
           !x.is_non_overlapping_and_dense())
-        return py::none();
+        return nullptr;
       if (device < 0) device = x.get_device();
-      if (x.get_device() != device) return py::none();
+      if (x.get_device() != device) return nullptr;
       int32_t code;
       switch (x.scalar_type()) {  // include/dlagg.h DLA_*
         case at::kFloat: code = 0; break;
         case at::kBFloat16: code = 1; break;
         case at::kHalf: code = 2; break;
         case at::kDouble: code = 3; break;
-        default: return py::none();
+        default: return nullptr;
       }
       if (l == 0) {
-        codes[t] = code;
-        numels[t] = x.numel();
-        wide = wide || code == 3;
+        tables->codes[t] = code;
+        tables->numels[t] = x.numel();
+        tables->wide = tables->wide || code == 3;
       } else {
-        const at::Tensor& x0 = THPVariable_Unpack(PyList_GET_ITEM(first, t));
-        if (code != codes[t] || x.sizes() != x0.sizes()) return py::none();
-        if (x.strides() != x0.strides() && !(x.is_contiguous() && x0.is_contiguous())) return py::none();
+        const at::Tensor& x0 = THPVariable_Unpack(lists[0][t]);
+        if (code != tables->codes[t] || x.sizes() != x0.sizes()) return nullptr;
+        if (x.strides() != x0.strides() && !(x.is_contiguous() && x0.is_contiguous())) return nullptr;
       }
       const uint64_t p = x.numel() ? reinterpret_cast<uint64_t>(x.data_ptr()) : 0;
       if (l < lead) {
-        head[l * n + t] = p;
+        tables->head[l * n + t] = p;
       } else {
-        tail[t * rest + (l - lead)] = p;
+        tables->tail[t * rest + (l - lead)] = p;
       }
     }
   }
+  tables->device = device;
+  return tables;
+}
+
+// pack_lists of Python lists, or None (the caller's own pass then says which tensor does not fit, or copies it).
+// The tensors of lists[bump] (-1: none) are about to be written: their version counters move on, as torch's own
+// in-place operators do it.
+py::object dense_lists(py::list lists, py::ssize_t lead, py::ssize_t bump) {
+  const py::ssize_t n_lists = PyList_GET_SIZE(lists.ptr());
+  if (n_lists < 1 || lead < 1 || lead > n_lists) return py::none();
+  std::vector<std::vector<PyObject*>> all(n_lists);
+  for (py::ssize_t l = 0; l < n_lists; ++l) {
+    PyObject* list = PyList_GET_ITEM(lists.ptr(), l);
+    if (!PyList_Check(list)) return py::none();
+    const py::ssize_t n = PyList_GET_SIZE(list);
+    all[l].resize(n);
+    for (py::ssize_t t = 0; t < n; ++t) all[l][t] = PyList_GET_ITEM(list, t);
+  }
+  if (all[0].empty()) return py::none();
+  auto tables = pack_lists(all, static_cast<size_t>(lead));
+  if (!tables) return py::none();
   if (bump >= 0 && bump < n_lists) {
-    PyObject* list = PyList_GET_ITEM(lists.ptr(), bump);
-    for (py::ssize_t t = 0; t < n; ++t) {
-      const at::Tensor& x = THPVariable_Unpack(PyList_GET_ITEM(list, t));
+    for (PyObject* o : all[bump]) {
+      const at::Tensor& x = THPVariable_Unpack(o);
       if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
     }
   }
   return py::cast(std::move(tables));
+}
+
+// pack_lists of the parameters of modules (parameters() order), the first of them ahead of the others; None when a
+// tree holds a class outside `plain`, when there are no parameters, or when pack_lists has none.
+py::object module_tables(py::list models, py::object plain) {
+  const py::ssize_t n = PyList_GET_SIZE(models.ptr());
+  if (n < 1 || !PySet_Check(plain.ptr())) return py::none();
+  std::vector<std::vector<PyObject*>> all(n);
+  PtrSet seen_m, seen_p;
+  for (py::ssize_t m = 0; m < n; ++m) {
+    seen_m.clear();
+    seen_p.clear();
+    if (!walk(PyList_GET_ITEM(models.ptr(), m), plain.ptr(), seen_m, seen_p, all[m])) return py::none();
+  }
+  if (all[0].empty()) return py::none();
+  auto tables = pack_lists(all, 1);
+  return tables ? py::cast(std::move(tables)) : py::object(py::none());
 }
 
 // (addresses, byte lengths) of a list of byte blocks as two int64 arrays — the block list an EVA transfer
@@ -1654,12 +1755,12 @@ PYBIND11_MODULE(_dla_walk, m) {
   py::class_<DenseTables>(m, "DenseTables")
       .def_readonly("n", &DenseTables::n)
       .def_readonly("device", &DenseTables::device)
-      .def_readonly("wide", &DenseTables::wide)
-      .def_property_readonly("codes", &DenseTables::codes_at)
-      .def_property_readonly("numels", &DenseTables::numels_at)
-      .def_property_readonly("rest", &DenseTables::rest_at)
-      .def("lead", &DenseTables::lead_at);
+      .def("norm", &DenseTables::norm)
+      .def("clip", &DenseTables::clip)
+      .def("peer_norms", &DenseTables::peer_norms)
+      .def("bounded", &DenseTables::bounded);
   m.def("dense_lists", &dense_lists, py::arg("lists"), py::arg("lead"), py::arg("bump"));
+  m.def("module_tables", &module_tables, py::arg("models"), py::arg("plain"));
   m.def("block_table", &block_table, py::arg("blocks"));
   m.def("fingerprint", &fingerprint, py::arg("model"), py::arg("plain"));
   m.def("param_views", &param_views, py::arg("flat"), py::arg("params"), py::arg("offsets"), py::arg("memo"));

@@ -586,6 +586,25 @@ def test_norm_bounded_fedavg(device, dtype, gains, own_center):
     _check_module(out, models, center, [0.2] * 5, 3.0, device)
 
 
+@pytest.mark.parametrize("device", ["cpu", "cuda:0"])
+def test_norm_bounded_fedavg_of_channels_last_models(device):
+    """Models whose parameters have another element order, all of them or one of them."""
+    from accdfl_amd.core.gradient_aggregation.norm_bounded import NormBoundedFedAvg
+
+    for orders in ((True, True, True, True), (True, False, True, False), (False, True, True, False)):
+        models = []
+        for k, last in enumerate(orders):
+            torch.manual_seed(k)
+            net = nn.Sequential(nn.Conv2d(4, 6, 3), nn.BatchNorm2d(6), nn.Conv2d(6, 5, 3, bias=False)).to(device)
+            models.append(net.to(memory_format=torch.channels_last) if last else net)
+        center = models.pop()
+        out = NormBoundedFedAvg(1.0, center).aggregate(models, [0.2, 0.3, 0.5])
+        want, _, added = no.bounded([list(m.parameters()) for m in models], [0.2, 0.3, 0.5], list(center.parameters()), 1.0)
+        for o, w, a, p in zip(out.parameters(), want, added, models[0].parameters()):
+            assert o.stride() == p.stride() and o.device == p.device
+            no.assert_close(o, w, 1000, a)
+
+
 def test_norm_bounded_fedavg_of_models_in_two_places():
     from accdfl_amd.core.gradient_aggregation.norm_bounded import NormBoundedFedAvg
 
