@@ -1121,7 +1121,10 @@ int round_impl(const char* what, const Round& r, double max_norm, const double* 
   if (!sq_in && m > 0) {
     // peers beside one read of the centre: 8 at most (their loads are all in flight), groups of equal size
     const int groups = (n + 7) / 8, g = (n + groups - 1) / groups;
-    blocks = std::min<int64_t>(norm_units, std::max<int64_t>(1, kPeerBlocks / groups));
+    // from 5 groups on, as many workgroups as run at once (2 per CU): 128 x 21.3 M bf16 852 us, 871 with twice as
+    // many; with fewer groups the second half evens out the first (16 x ResNet-34 bf16 127, 131 with half)
+    const int most = groups > 4 ? kPeerBlocks / 2 : kPeerBlocks;
+    blocks = std::min<int64_t>(norm_units, std::max<int64_t>(1, most / groups));
     // large rounds join in a kernel of its own: its launch hides behind the round, the last workgroup's join does
     // not (us, apart / in the last workgroup: 8 x 25 M f32 138.6 / 141.6; but 2 x 85 K f32 with the average 15.5 / 12.7)
     if (blocks * groups > kPeerBlocks / 2) counters = nullptr;
