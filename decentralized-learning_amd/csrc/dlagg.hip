@@ -204,7 +204,7 @@ template <> struct Ops<DLA_BF16> {
 
 // Two bf16 FedAvg steps on one 32-bit word of two bf16 values (element 0 in the low half):
 // acc[e] = R(acc[e] + R(w * x[e])), R = RNE to bf16, op-math fp32 — Ops<DLA_BF16>::step on
-// both elements, with packed fp32 ops and one conversion per element per rounding
+// both elements, as pairs with one conversion per element per rounding
 // (round_bf16: 8 VALU per word and step against 10 for one packed conversion + shift + mask).
 __device__ inline f32x2 round_bf16x2(f32x2 v) { return f32x2{round_bf16(v.x), round_bf16(v.y)}; }
 __device__ inline void bf16_step2(float& a0, float& a1, float w, uint32_t word) {
@@ -239,7 +239,7 @@ __device__ inline float pin(float f) {
 __device__ inline float round_f16(float f) { return static_cast<float>(static_cast<_Float16>(pin(f))); }
 
 // Two f16 FedAvg steps on one 32-bit word of two f16 values (element 0 in the low half), as
-// Ops<DLA_F16>::step on both: packed fp32 multiply / add, one v_cvt_pk_f16_f32 (RNE) per
+// Ops<DLA_F16>::step on both: multiply / add of pairs, one v_cvt_pk_f16_f32 (RNE) per
 // rounding.  The product and the sum are pinned as rounded fp32 pairs first, for the same
 // reason as pin(): no fused mix-precision form may skip the fp32 rounding.
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -338,7 +338,7 @@ __device__ inline void store16(uint4* p, const uint4& v) {
 // ACC_IN: the running sum starts from `out` (second and later passes of a reduce
 // with more than KMAX peers) instead of p0 * 0.
 // One peer's 16-byte chunk folded into its E running sums (fedavg.py:22 when `first`, then
-// fedavg.py:25).  PK: 16-bit pairs through bf16_step2 / f16_step2 (packed fp32 ops, one
+// fedavg.py:25).  PK: 16-bit pairs through bf16_step2 / f16_step2 (pairs, one
 // packed conversion per rounding).  fold_tile uses it for peer tables of more than 8
 // (16 x 21.3 M bf16 121.9 -> 118.8 us, f16 168.3 -> 118.9) and for f16 groups of 8 with
 // smaller tables (8 x 50 M f16 191.8 -> 142.4).  bf16 tables of <= 8 peers and the
@@ -663,8 +663,7 @@ __device__ __attribute__((always_inline)) inline void fold_words(
   for (int g = 0; g < G; ++g) {
     if (FULL || g < m) {
       if constexpr (DT == DLA_BF16) {
-        // both bf16 elements of the word at once: v_pk_mul_f32 / v_pk_add_f32 and one
-        // v_cvt_pk_bf16_f32 per rounding (same per-element arithmetic as Ops::step)
+        // both bf16 elements of the word as a pair (same per-element arithmetic as Ops::step)
         if (!ACC_IN && g == 0 && first_round) {
           acc_t x[2];
           O::unpack_w(v[g], x);
