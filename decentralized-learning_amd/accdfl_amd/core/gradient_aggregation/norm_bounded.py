@@ -8,8 +8,8 @@ update is not finite adds nothing::
     n_k    = || p_k - c ||_2
     result = c + sum_k w_k min(1, max_norm / n_k) (p_k - c)
 
-With a bound above every norm and weights that add up to 1 this is the weighted average of the models, carried in
-64 bits and rounded once (FedAvg rounds every step, as the reference does).
+With a bound above every norm and weights that add up to 1 this is the weighted average of the models, rounded once
+(FedAvg rounds every step, as the reference does).
 
 The contract is FedAvg.aggregate's (weights, defaults, errors; the result is ``copy.deepcopy(models[0])`` with
 the averaged parameters, on models[0]'s device), selected by ``settings.gradient_aggregation =
@@ -18,8 +18,10 @@ and the centre must have the same parameters (count, shapes, dtypes).
 """
 from __future__ import annotations
 
-from typing import List, Optional
+import threading
+from typing import Dict, List, Optional
 
+import numpy as np
 import torch
 from torch import nn
 
@@ -60,6 +62,117 @@ def _device_round(models: List[nn.Module], weights, center: nn.Module, max_norm:
         return _fedavg._clone_value(models[0], memo)
 
 
+class _HostStage:
+    """Two page-locked buffers that CPU models go through on their way to one GPU and the average on its way back, each
+    with the event after the copy that last used it, and the stream of those copies."""
+
+    BYTES = 32 << 20
+
+    def __init__(self, device: torch.device):
+        self.buffers = [torch.empty(self.BYTES, dtype=torch.uint8, pin_memory=True) for _ in range(2)]
+        self.events: List[Optional[torch.cuda.Event]] = [None, None]
+        self.stream = torch.cuda.Stream(device)
+
+    def wait(self, i: int) -> torch.Tensor:
+        if self.events[i] is not None:
+            self.events[i].synchronize()
+        return self.buffers[i]
+
+    def copy(self, i: int, dst: torch.Tensor, src: torch.Tensor, stream: torch.cuda.Stream) -> None:
+        with torch.cuda.stream(stream):
+            dst.copy_(src, non_blocking=True)
+            self.events[i] = torch.cuda.Event()
+            self.events[i].record(stream)
+
+
+_host_stages: Dict[torch.device, _HostStage] = {}
+_host_lock = threading.Lock()
+
+
+def release_staging() -> None:
+    """Free the page-locked buffers of CPU rounds."""
+    with _host_lock:
+        _host_stages.clear()
+
+
+class _Pieces:
+    """Host tensors (addresses row by row, each row the tensors of ``numels``) that lie in device memory row after row,
+    ``pitch`` bytes apart: what of them falls into a range of those bytes."""
+
+    def __init__(self, ptrs, numels: List[int], esize: int, pitch: int):
+        sizes = np.array(numels, dtype=np.int64) * esize
+        rows = len(ptrs) // len(numels)
+        starts = ((np.cumsum(sizes) - sizes)[None, :] + np.arange(rows, dtype=np.int64)[:, None] * pitch).reshape(-1)
+        sizes = np.tile(sizes, rows)
+        some = sizes > 0
+        self.ptrs = np.array(ptrs, dtype=np.int64)[some]
+        self.starts = starts[some]
+        self.ends = self.starts + sizes[some]
+        self.end = int(self.ends[-1]) if len(self.ends) else 0
+
+    def within(self, a: int, b: int):
+        """(host addresses, offsets from ``a``, byte counts) of the pieces in [a, b)."""
+        lo, hi = int(np.searchsorted(self.ends, a, side="right")), int(np.searchsorted(self.starts, b, side="left"))
+        begin = np.maximum(self.starts[lo:hi], a)
+        return self.ptrs[lo:hi] + (begin - self.starts[lo:hi]), begin - a, np.minimum(self.ends[lo:hi], b) - begin
+
+
+def _host_round(models: List[nn.Module], weights, center: nn.Module, max_norm: float) -> Optional[nn.Module]:
+    """The round of CPU models of one layout and dtype: every model goes to the GPU once, as a flat row — packed 32 MiB
+    at a time by the library's threaded copy into one page-locked buffer while the other's DMA runs — and the average
+    comes back the same way.  None when the models do not qualify."""
+    own = center is not models[0]
+    layout = _fedavg._host_layout(([center] if own else []) + models)
+    if layout is None:
+        return None
+    dtype, numels, ptrs = layout
+    total, rows = sum(numels), len(models) + own
+    if total == 0:
+        return None
+    device = _wsum.require_device(None)
+    esize = torch.empty((), dtype=dtype).element_size()
+    pitch = (total * esize + 255) // 256 * 256
+    ingress = _Pieces(np.frombuffer(ptrs, dtype=np.int64), numels, esize, pitch)
+    cur = torch.cuda.current_stream(device)
+    buf = torch.empty(rows * pitch, dtype=torch.uint8, device=device)
+    with _host_lock:
+        stage = _host_stages.get(device)
+        if stage is None:
+            stage = _host_stages[device] = _HostStage(device)
+        stream = cur if ingress.end <= stage.BYTES else stage.stream  # one piece: nothing to overlap
+        stream.wait_stream(cur)
+        try:
+            for i, a in enumerate(range(0, ingress.end, stage.BYTES)):
+                b = min(ingress.end, a + stage.BYTES)
+                host = stage.wait(i & 1)
+                at, off, n = ingress.within(a, b)
+                _lib.host_copy_batch(host.data_ptr() + off, at, n, streaming=True)
+                stage.copy(i & 1, buf[a:b], host[: b - a], stream)
+            result = _fedavg._center_copy(models[0])  # while the last copies run
+            params = list(result.parameters())
+            if len(params) != len(numels) or not all(p.is_cpu and p.is_contiguous() for p in params):
+                return None
+            cur.wait_stream(stream)
+            flat = buf.view(dtype)
+            peers = [flat[k * (pitch // esize):][:total] for k in range(rows)]
+            out, _ = _norms.wsum_bounded(peers[own:], weights, peers[0], max_norm)
+            out = out.view(torch.uint8)
+            egress = _Pieces([p.data_ptr() for p in params], numels, esize, pitch)
+            stream.wait_stream(cur)
+            pieces = [(a, min(egress.end, a + stage.BYTES)) for a in range(0, egress.end, stage.BYTES)]
+            for i in range(len(pieces) + 1):
+                if i < len(pieces):
+                    a, b = pieces[i]
+                    stage.copy(i & 1, stage.wait(i & 1)[: b - a], out[a:b], stream)
+                if i > 0:
+                    a, b = pieces[i - 1]
+                    at, off, n = egress.within(a, b)
+                    _lib.host_copy_batch(at, stage.wait((i - 1) & 1).data_ptr() + off, n)
+        finally:
+            cur.wait_stream(stream)  # what follows on the caller's stream may take this round's memory
+    return result
+
+
 def _check_layout(models: List[nn.Module], center: nn.Module) -> List[List[torch.Tensor]]:
     """The parameters of the centre and of every model; raises unless all have models[0]'s."""
     lists = [_fedavg._parameters(m) for m in [center] + models]
@@ -76,8 +189,8 @@ def _check_layout(models: List[nn.Module], center: nn.Module) -> List[List[torch
 
 
 def _general_round(models: List[nn.Module], weights, center: nn.Module, max_norm: float) -> nn.Module:
-    """Any other round (CPU models, models on several devices, parameters of several dtypes): everything is
-    brought to models[0]'s GPU (the current one for CPU models), averaged there and copied into the result."""
+    """Any other round (models on several devices, parameters of several dtypes): everything is brought to models[0]'s
+    GPU (the current one for CPU models), averaged there and copied into the result."""
     lists = _check_layout(models, center)
     result = _fedavg._center_copy(models[0])
     params = list(result.parameters())
@@ -85,14 +198,6 @@ def _general_round(models: List[nn.Module], weights, center: nn.Module, max_norm
         return result
     home = params[0].device
     device = _wsum.require_device(home if home.type == "cuda" else None)
-    if len({p.dtype for p in params}) == 1 and all(p.device.type == "cpu" for ps in lists for p in ps):
-        from accdfl_amd.core.peer_slab import PeerSlab
-
-        slab = PeerSlab([p.shape for p in params], params[0].dtype, len(models), device)
-        for ps in lists[1:]:
-            slab.stage(ps)
-        slab.reduce_bounded_into(params, max_norm, weights, center=None if center is models[0] else lists[0])
-        return result
     resident = [[p.detach().to(device) for p in ps] for ps in lists]
     outs = [torch.empty_like(p) for p in resident[0]]
     _norms.wsum_bounded_multi(resident[1:], weights, resident[0], max_norm, outs)
@@ -119,5 +224,7 @@ class NormBoundedFedAvg(GradientAggregation):
         _norms._check_peers(len(models))
         with torch.no_grad():
             center = self.center if self.center is not None else models[0]
-            done = _device_round(models, weights, center, self.max_norm)
+            first = next(iter(models[0].parameters()), None)
+            on_host = first is not None and first.is_cpu
+            done = (_host_round if on_host else _device_round)(models, weights, center, self.max_norm)
             return done if done is not None else _general_round(models, weights, center, self.max_norm)

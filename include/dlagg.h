@@ -227,7 +227,7 @@ int dla_mean(int dtype, const void* const* peers, int n_peers, int64_t n_elems, 
 /* ---- norms over many tensors, and what is bounded by them (additive in ABI v13) ----
  *
  * Tensors are dense and of any of the four dtypes, mixed freely within a call; their pointers need element
- * alignment only.  Sums and norms are carried in 64 bits.  Nothing synchronises; the stream's device must be
+ * alignment only.  The sums of norms are carried in 64 bits.  Nothing synchronises; the stream's device must be
  * current.  Without a table_host, launches take everything by value except the caller's buffers, so a captured call
  * replays.  The workspaces are the caller's, need no initialisation and hold nothing between calls; two calls in
  * flight at once need two.  The counters (NULL: one launch more) let a kernel's last workgroup add up what the others
@@ -278,8 +278,8 @@ int dla_peer_norms(int n_tensors, const int* dtypes, const void* const* peer_ptr
 
 /* fedavg.py:20-25 with every peer's update bounded first:
  *     out = round(c + sum_k a_k (p_k - c)),   a_k = weights[k] * (n_k <= max_norm ? 1 : max_norm / n_k)
- * with n_k as dla_peer_norms gives it, in list order, carried in 64 bits and rounded once (dla_wsum rounds every
- * step, as the reference does).  A peer whose n_k is not finite adds nothing and is not read.  outs[t] may be
+ * with n_k as dla_peer_norms gives it, in list order, carried in 64 bits (32 for BF16 and F16) and rounded once
+ * (dla_wsum rounds every step, as the reference does).  A peer whose n_k is not finite adds nothing and is not read.  outs[t] may be
  * tensor t of the centre or of a peer; every other overlap is refused (DLA_E_ALIAS).
  *   sq  DEVICE doubles [n_peers], the squared norms to bound by (a bucket of a model whose norms are known), or
  *       NULL: computed here */

@@ -1,9 +1,12 @@
 """The norm and clipping operators from their definitions, in 64 bits on the CPU (test infrastructure only), and how
 far a correct result may be from them.
 
-Every result is carried in 64 bits and rounded once (16-bit types through float32), so with u = eps / 2 of the
-storage type, v = 2^-24 (0 for float64) and w = 2^-53 * terms for the 64-bit sums,
-    |got - want| <= (u + v) |want| + w * (sum of the magnitudes added) + half the smallest subnormal."""
+Norms, products and averages are carried in 64 bits and rounded once (16-bit types through float32), so with u = eps / 2
+of the storage type, v = 2^-24 (0 for float64) and w = 2^-53 * terms for the 64-bit sums,
+    |got - want| <= (u + v) |want| + w * (sum of the magnitudes added) + half the smallest subnormal.
+The averages of 16-bit types are carried in 32 bits: c + sum_k a_k d_k over N peers rounds a_k and d_k once each (2 * 2^-24 of
+|a_k d_k|), every one of the N fused additions (2^-24 of a partial sum, at most M = |c| + sum_k |a_k d_k|) and the
+addition of c (2^-24 M): at most (N + 3) 2^-24 M, beside the terms above."""
 import math
 
 import numpy as np
@@ -49,7 +52,7 @@ def shares(norms, weights, max_norm):
 
 
 def bounded(models, weights, center, max_norm, norms=None):
-    """(results, norms, the magnitudes added for each result)."""
+    """(results, norms, (N + 3) M for each result)."""
     if norms is None:
         norms = update_norms(models, center)
     outs, added = [], []
@@ -62,7 +65,7 @@ def bounded(models, weights, center, max_norm, norms=None):
             d = a * (ms[i].detach().cpu().to(torch.float64) - c)
             acc, mag = acc + d, mag + d.abs()
         outs.append(c + acc)
-        added.append(mag)
+        added.append(mag * (len(models) + 3))
     return outs, norms, added
 
 
@@ -89,6 +92,8 @@ def assert_close(got, want, terms, added=None):
     v = 0.0 if got.dtype == torch.float64 else 2.0 ** -24
     mag = want.abs() if added is None else added
     tol = (info.eps / 2 + v) * want.abs() + 2.0 ** -53 * (terms + 16) * mag + info.smallest_normal * info.eps / 2
+    if added is not None and got.dtype in (torch.bfloat16, torch.float16):
+        tol = tol + 2.0 ** -24 * added
     fine = torch.isfinite(want) & (want.abs() <= info.max)
     bad = fine & ~((g - want).abs() <= tol)
     assert not bool(bad.any()), "%d of %d differ, worst %g at tolerance %g" % (

@@ -613,6 +613,38 @@ def test_norm_bounded_fedavg_of_models_in_two_places():
     _check_module(NormBoundedFedAvg(3.0, center.cpu()).aggregate(models, weights), models, center, weights, 3.0, "cuda:0")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("own_center", [False, True])
+def test_norm_bounded_fedavg_of_large_cpu_models(dtype, own_center):
+    """Rows beyond one page-locked buffer, tensors cut at its end, empty tensors, two calls at once."""
+    from accdfl_amd.core.gradient_aggregation import norm_bounded
+
+    def model(seed):
+        g = torch.Generator().manual_seed(seed)
+        return nn.ParameterList([nn.Parameter((torch.randn(s, generator=g) * 0.1).to(dtype))
+                                 for s in ((3, 5), (0,), (2_000_003,), (7,), (1500, 2001), (1,))])
+
+    models, center = [model(k) for k in range(4)], model(50)
+    weights = [0.4, 0.3, 0.2, 0.1]
+    c = center if own_center else models[0]
+    want, _, added = no.bounded([list(m) for m in models], weights, list(c), 200.0)
+    outs = [None, None]
+
+    def work(i):
+        outs[i] = norm_bounded.NormBoundedFedAvg(200.0, center if own_center else None).aggregate(models, weights)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(100)
+    for out in outs:
+        for o, w, a in zip(out, want, added):
+            assert o.is_cpu
+            no.assert_close(o, w, 5_001_530, a)
+    norm_bounded.release_staging()
+
+
 @pytest.mark.parametrize("with_model", [False, True])
 def test_managers(with_model):
     """Both managers, the registry's order; the device manager's round runs over its staged slab rows."""
