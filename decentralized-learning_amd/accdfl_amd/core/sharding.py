@@ -125,6 +125,8 @@ class BucketShardedFedAvg:
             weights = [float(1. / n) for _ in range(n)]
         else:
             assert len(weights) == n
+        if not float(max_norm) >= 0.0:  # before the collective, on ranks with an empty bucket too
+            raise ValueError("max_norm must be >= 0, got %r" % (max_norm,))
         start, end = self.local_range
         m = end - start
         sq = self.update_sq_norms(peer_buckets, center_bucket)
