@@ -16,10 +16,11 @@ of a model once before the first element can be written, which is what these ope
 Tensors are float32 / bfloat16 / float16 / float64, mixed freely within a list, on one HIP device, empty ones
 included.  Dense tensors are read where they are whatever the order of their axes and wherever they start; others
 (a slice with gaps, an expanded tensor) are copied first.  Norms and products are carried in 64 bits, averages in 64
-(32 for the 16-bit types), and rounded once.  Results are on the device and nothing synchronises; nothing here is differentiable.  Work is
-enqueued on ``stream`` or the current stream of the tensors' device, workspaces come from torch's caching
-allocator for each call, and every launch takes its tables by value: calls on several streams or threads do not
-meet, and a call captured into a graph replays.
+(32 for the 16-bit types), and rounded once.  Results are on the device and nothing synchronises; nothing here is
+differentiable.  Work is enqueued on ``stream`` or the current stream of the tensors' device, workspaces come from
+torch's caching allocator for each call, and launches take their tables by value (those of large rounds from a slot
+of page-locked memory that the call owns until the GPU has read it; under capture by value too): calls on several
+streams or threads do not meet, and a call captured into a graph replays.
 """
 from __future__ import annotations
 
@@ -328,7 +329,8 @@ def clip_global_norm_(tensors: Tensors, max_norm: float, norm_type: float = 2.0,
 def clip_grad_norm_(parameters: Tensors, max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_'s contract: the gradients of ``parameters`` (parameters, or a module) clipped
-    in place by their global norm, which is returned.  Parameters without a gradient are skipped."""
+    in place by their global norm, which is returned.  Parameters without a gradient are skipped; the gradients
+    are on one device, dense and distinct."""
     grads = [p.grad for p in _tensors_of(parameters)]
     return clip_global_norm_([g for g in grads if g is not None], max_norm, norm_type, error_if_nonfinite)
 
@@ -420,10 +422,11 @@ def wsum_bounded_multi(peer_params: Sequence[Tensors], weights: Sequence[float],
         n_k     = || peer_k - center ||_2  over all its tensors
         outs[i] = center[i] + sum_k weights[k] * min(1, max_norm / n_k) * (peer_k[i] - center[i])
 
-    in list order, carried in 64 bits (32 for the 16-bit types) and rounded once.  A peer whose update is not finite (n_k is NaN or infinite)
-    adds nothing.  ``outs[i]`` may be the i-th tensor of the centre or of a peer; no other overlap.  ``sq_norms``:
-    float64 squared norms [n] on the device to bound by, when the tensors are one bucket of models whose norms are
-    known (update_norms(squared=True), added up).  Returns the norms [n], float32 (float64 if any tensor is)."""
+    in list order, carried in 64 bits (32 for the 16-bit types) and rounded once.  A peer whose update is not
+    finite (n_k is NaN or infinite) adds nothing.  ``outs[i]`` may be the i-th tensor of the centre or of a peer; no
+    other overlap.  ``sq_norms``: float64 squared norms [n] on the device to bound by, when the tensors are one
+    bucket of models whose norms are known (update_norms(squared=True), added up).  At most 2 048 peers.  Returns
+    the norms [n], float32 (float64 if any tensor is)."""
     bound = _bound(max_norm)
     outs = _tensors_of(outs)
     lists = [_tensors_of(center_params), outs] + [_tensors_of(p) for p in peer_params]

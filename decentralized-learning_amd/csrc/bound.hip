@@ -15,10 +15,11 @@
 // for the 16-bit types (Average below).  A result is rounded to its storage type once (16-bit types through
 // f32: the first rounding moves a result by at most 2^-24 of itself).
 //
-// Work is cut into units of 1 to 32 KiB of one tensor; a unit never spans tensors.  Workgroup b of P takes units b, b + P, b + 2 P, ...: the chip walks every
-// stream as one front (few DRAM rows and pages at a time), and there is one partial result per workgroup
-// whatever the size, added up in a fixed order by the kernel that needs the sum, so the results do not
-// depend on which workgroup ended first.  Loads need element alignment only (gfx950
+// Work is cut into units of 1 to 32 KiB of one tensor; a unit never spans tensors.  The norms deal them round
+// robin to P workgroups, the kernels that write give each a workgroup of its own in order: either way the chip
+// walks every stream as one front (few DRAM rows and pages at a time; ranges instead of round robin cost 9 %
+// for 128 peers).  A norm has one partial result per workgroup whatever the size, and they are joined in a fixed
+// order, so results do not depend on which workgroup ended first.  Loads need element alignment only (gfx950
 // takes 16-byte loads from any address), so tensors that start anywhere take the same path.
 #include <hip/hip_runtime.h>
 
@@ -27,6 +28,7 @@
 #include <cstdint>
 #include <cstring>
 #include <exception>
+#include <new>
 #include <string>
 #include <type_traits>
 #include <utility>
@@ -470,10 +472,11 @@ struct Layout {      // where element j of a peer (and of the centre) lies, in e
   int64_t stride;
   int64_t center_stride;
 };
-constexpr int kPeerVec = 4;                             // 16-byte loads of one peer in a row per lane
-constexpr int kNormUnit = kThreads * 16;                // bytes of one tensor of one peer, times 1 or kPeerVec
-constexpr int kMeanThreads = 64, kMeanSteps = 1;
-constexpr int kMeanUnit = kMeanThreads * 16 * kMeanSteps;
+// 16-byte loads of one peer in a row per lane of the norms: 16 KiB of each stream at a time (8 x 25 M f32 138 us, with
+// one load 143); tiles of a slab lie side by side anyway.
+constexpr int peer_vec(bool tiled) { return tiled ? 1 : 4; }
+constexpr int kMeanThreads = 64;                        // the average: one wave, 1 KiB of each stream
+constexpr int kMeanUnit = kMeanThreads * 16;
 constexpr int kPutWords = 480;
 struct PutWords {
   uint64_t w[kPutWords];
@@ -526,10 +529,10 @@ __device__ inline int find_seg(const Seg* segs, int count, int64_t u) {
   return lo;
 }
 
-template <int DT, int G, int V, bool TILED>
+template <int DT, int G, bool TILED>
 __device__ inline void peer_norm_unit(const Layout& l, const void* center, const void* const (&p)[G], int64_t n,
                                       int64_t unit, double (&acc)[G]) {
-  constexpr int E = Elem<DT>::E;
+  constexpr int E = Elem<DT>::E, V = peer_vec(TILED);
   const int64_t j0 = unit * (kThreads * V * E) + static_cast<int>(threadIdx.x) * E;
   u32x4 rc[V], r[G][V];
   if ((unit + 1) * (kThreads * V * E) <= n) {
@@ -599,7 +602,7 @@ __device__ inline void join_peer(const double* partials, int n, int k, const dou
 // partials[k * gridDim.x + b]: workgroup b's part of || p_k - c ||^2 for the peers of group blockIdx.y.  G
 // peers are read beside one read of the centre, so the centre costs 1 / G of a peer.  With counters (one per
 // group), a group's last workgroup joins its peers.
-template <int G, int V, bool TILED>
+template <int G, bool TILED>
 __global__ __launch_bounds__(kThreads) void peer_norms_kernel(const PutWords words, Table tab, int64_t units, Layout l,
                                                               double* partials, uint32_t* counters, const Joined to) {
   __shared__ double lds[kWaves];
@@ -630,10 +633,10 @@ __global__ __launch_bounds__(kThreads) void peer_norms_kernel(const PutWords wor
       }
     }
     switch (dt) {
-      case DLA_F32: peer_norm_unit<DLA_F32, G, V, TILED>(l, center, p, n, u - first, acc); break;
-      case DLA_BF16: peer_norm_unit<DLA_BF16, G, V, TILED>(l, center, p, n, u - first, acc); break;
-      case DLA_F16: peer_norm_unit<DLA_F16, G, V, TILED>(l, center, p, n, u - first, acc); break;
-      default: peer_norm_unit<DLA_F64, G, V, TILED>(l, center, p, n, u - first, acc); break;
+      case DLA_F32: peer_norm_unit<DLA_F32, G, TILED>(l, center, p, n, u - first, acc); break;
+      case DLA_BF16: peer_norm_unit<DLA_BF16, G, TILED>(l, center, p, n, u - first, acc); break;
+      case DLA_F16: peer_norm_unit<DLA_F16, G, TILED>(l, center, p, n, u - first, acc); break;
+      default: peer_norm_unit<DLA_F64, G, TILED>(l, center, p, n, u - first, acc); break;
     }
   }
 #pragma unroll
@@ -684,34 +687,31 @@ __device__ inline void mean_unit(const Layout& l, const uint64_t* ptrs, const do
                                  const void* center, void* out, int64_t n, int64_t unit) {
   using A = Average<DT>;
   constexpr int E = Elem<DT>::E;
-  const bool full = (unit + 1) * (kMeanThreads * kMeanSteps * E) <= n;
-#pragma unroll 1
-  for (int step = 0; step < kMeanSteps; ++step) {
-    const int64_t j = (unit * kMeanSteps + step) * (kMeanThreads * E) + static_cast<int>(threadIdx.x) * E;
-    const int64_t at = place<TILED>(l, l.stride, j), at_c = place<TILED>(l, l.center_stride, j);
-    const int part = full ? E : clamp_part(n - j, E);
-    const u32x4 rc = full ? load_full<DT>(center, at_c) : load_part<DT>(center, at_c, part);
-    typename A::real c[E], acc[E] = {};
-    Elem<DT>::widen(rc, c);
+  const int64_t j = unit * (kMeanThreads * E) + static_cast<int>(threadIdx.x) * E;
+  const int64_t at = place<TILED>(l, l.stride, j), at_c = place<TILED>(l, l.center_stride, j);
+  const bool full = (unit + 1) * (kMeanThreads * E) <= n;
+  const int part = full ? E : clamp_part(n - j, E);
+  const u32x4 rc = full ? load_full<DT>(center, at_c) : load_part<DT>(center, at_c, part);
+  typename A::real c[E], acc[E] = {};
+  Elem<DT>::widen(rc, c);
 #pragma unroll
-    for (int e = 0; e < E; ++e) c[e] = A::center(c[e]);
-    int i = 0;
-    for (; i + 8 <= n_peers; i += 8) fold_peers<DT, 8, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
-    if (i + 4 <= n_peers) {
-      fold_peers<DT, 4, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
-      i += 4;
-    }
-    if (i + 2 <= n_peers) {
-      fold_peers<DT, 2, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
-      i += 2;
-    }
-    if (i < n_peers) fold_peers<DT, 1, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
-    Elem<DT>::widen(rc, c);
-    // where the centre is not finite no peer counts, and the centre stays
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = __builtin_isfinite(c[e]) ? acc[e] + c[e] : c[e];
-    store_part<DT>(out, j, part, Elem<DT>::narrow(acc));
+  for (int e = 0; e < E; ++e) c[e] = A::center(c[e]);
+  int i = 0;
+  for (; i + 8 <= n_peers; i += 8) fold_peers<DT, 8, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
+  if (i + 4 <= n_peers) {
+    fold_peers<DT, 4, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
+    i += 4;
   }
+  if (i + 2 <= n_peers) {
+    fold_peers<DT, 2, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
+    i += 2;
+  }
+  if (i < n_peers) fold_peers<DT, 1, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
+  Elem<DT>::widen(rc, c);
+  // where the centre is not finite no peer counts, and the centre stays
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = __builtin_isfinite(c[e]) ? acc[e] + c[e] : c[e];
+  store_part<DT>(out, j, part, Elem<DT>::narrow(acc));
 }
 
 // out = round(c + sum_k a_k (p_k - c)).  Units are dealt from the last to the first: what the norms read last is
@@ -741,13 +741,15 @@ __global__ __launch_bounds__(kMeanThreads) void bounded_kernel(const PutWords wo
 
 // ------------------------------------------------------------------ host side
 int fail(int code, const std::string& msg) { return dla_internal_fail(code, msg.c_str()); }
-int hip_fail(const char* what, hipError_t e) { return fail(static_cast<int>(e), std::string(what) + ": " + hipGetErrorString(e)); }
+int hip_fail(const char* what, hipError_t e) {
+  return fail(static_cast<int>(e), std::string(what) + ": " + hipGetErrorString(e)); }
 
 bool known_dtype(int dt) { return dt == DLA_F32 || dt == DLA_BF16 || dt == DLA_F16 || dt == DLA_F64; }
 bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 // No element count here exceeds this: 2^56 bytes, far beyond any device, keeps every product below in 64 bits.
 constexpr int64_t kMostElems = int64_t{1} << 53;
+constexpr double kInfinityCache = 256.0 * (1 << 20);
 
 // The launches a list of tensors takes: tensors [begin, end) of `order` (the non-empty ones), `units` units on
 // `blocks` workgroups.
@@ -800,8 +802,10 @@ int check_list(const char* what, int n_tensors, const int* dtypes, const void* c
   if (norm != DLA_NORM_L2 && norm != DLA_NORM_L1 && norm != DLA_NORM_INF)
     return fail(DLA_E_INVALID, std::string(what) + ": unknown norm " + std::to_string(norm));
   for (int t = 0; t < n_tensors; ++t) {
-    if (!known_dtype(dtypes[t])) return fail(DLA_E_INVALID, std::string(what) + ": tensor " + std::to_string(t) + " has unknown dtype " + std::to_string(dtypes[t]));
-    if (numels[t] < 0 || numels[t] > kMostElems) return fail(DLA_E_INVALID, std::string(what) + ": tensor " + std::to_string(t) + " has a bad element count");
+    if (!known_dtype(dtypes[t]))
+      return fail(DLA_E_INVALID, std::string(what) + ": tensor " + std::to_string(t) + " has unknown dtype " + std::to_string(dtypes[t]));
+    if (numels[t] < 0 || numels[t] > kMostElems)
+      return fail(DLA_E_INVALID, std::string(what) + ": tensor " + std::to_string(t) + " has a bad element count");
     if (numels[t] == 0) continue;
     if (!tensors[t] || !aligned_to(tensors[t], elem_bytes(dtypes[t])))
       return fail(DLA_E_INVALID, std::string(what) + ": tensor " + std::to_string(t) + " is null or not aligned to its elements");
@@ -903,7 +907,8 @@ int norm_impl(int n_tensors, const int* dtypes, const void* const* tensors, cons
   hipStream_t s = static_cast<hipStream_t>(stream);
   double* ws = static_cast<double*>(workspace);
   int n_partials = 0;
-  if (int rc = norm_launches("dla_norm", order, dtypes, tensors, numels, norm, true, out_dtype, out, counter, ws, &n_partials, s)) return rc;
+  if (int rc = norm_launches("dla_norm", order, dtypes, tensors, numels, norm, true, out_dtype, out, counter, ws, &n_partials, s))
+    return rc;
   return counter && n_partials > 0 ? DLA_OK : join_launch("dla_norm", norm, ws, n_partials, out_dtype, out, s);
 }
 
@@ -912,7 +917,7 @@ int norm_clip_impl(int n_tensors, const int* dtypes, const void* const* tensors,
                    int64_t workspace_bytes, void* stream) {
   std::vector<int> order;
   if (int rc = check_list("dla_norm_clip", n_tensors, dtypes, tensors, numels, norm, &order)) return rc;
-  if (!(max_norm >= 0) || !(eps >= 0)) return fail(DLA_E_INVALID, "dla_norm_clip: max_norm and eps must be >= 0");
+  if (!(max_norm >= 0) || !(eps > 0)) return fail(DLA_E_INVALID, "dla_norm_clip: max_norm must be >= 0 and eps > 0");
   if (int rc = check_norm_memory("dla_norm_clip", n_tensors, out_dtype, norm_out, counter, workspace, workspace_bytes)) return rc;
   if (!order.empty() && !outs) return fail(DLA_E_INVALID, "dla_norm_clip: null outs array");
   std::vector<Span> spans;
@@ -934,12 +939,13 @@ int norm_clip_impl(int n_tensors, const int* dtypes, const void* const* tensors,
     return fail(DLA_E_INVALID, "dla_norm_clip: too many elements");
   // What the Infinity Cache (256 MB) can hold is kept in the caches for the second read; more streams past them
   // (us, kept / streamed: 21 M bf16 27.4 / 30.8, 40 M f32 79.0 / 82.3; 0.87 G bf16 933 / 889)
-  int64_t bytes = 0;
-  for (int t : order) bytes += numels[t] * elem_bytes(dtypes[t]);
-  const bool nt = bytes > (int64_t{256} << 20);
+  double bytes = 0;
+  for (int t : order) bytes += static_cast<double>(numels[t]) * elem_bytes(dtypes[t]);
+  const bool nt = bytes > kInfinityCache;
   hipStream_t s = static_cast<hipStream_t>(stream);
   double* ws = static_cast<double*>(workspace);
-  if (int rc = norm_launches("dla_norm_clip", order, dtypes, tensors, numels, norm, nt, out_dtype, nullptr, counter, ws, &n_partials, s)) return rc;
+  if (int rc = norm_launches("dla_norm_clip", order, dtypes, tensors, numels, norm, nt, out_dtype, nullptr, counter, ws, &n_partials, s))
+    return rc;
   if (launches.empty()) return norm_out ? join_launch("dla_norm_clip", norm, ws, 0, out_dtype, norm_out, s) : DLA_OK;
   if (!counter)
     if (int rc = join_launch("dla_norm_clip", norm, ws, n_partials, DLA_F64, ws, s)) return rc;
@@ -959,14 +965,22 @@ int norm_clip_impl(int n_tensors, const int* dtypes, const void* const* tensors,
 }
 
 // ------------------------------------------------------------------ peers, host side
-constexpr int kPeerBlocks = 1024;  // workgroups of the norms: 4 per CU
 constexpr int kMostPeers = 2048;
+
+// Peers beside one read of the centre: 8 at most (their loads are all in flight), groups of equal size.  The norms
+// take 1 024 workgroups in all, from 5 groups on as many as run at once (2 per CU): 128 x 21.3 M bf16 852 us, 871
+// with twice as many; with fewer groups the second half evens out the first (16 x ResNet-34 bf16 127, 131 with half).
+int peer_groups(int n) { return (n + 7) / 8; }
+int64_t peer_blocks(int n) {
+  const int groups = peer_groups(n);
+  return std::max(1, (groups > 4 ? 512 : 1024) / groups);
+}
 
 int64_t peer_table_words(int64_t n_tensors, int64_t n_peers) {
   return n_tensors * static_cast<int64_t>(sizeof(Seg) / 8) + n_tensors * n_peers + n_peers;
 }
 int64_t peer_workspace_bytes(int64_t n_tensors, int64_t n_peers) {
-  return (peer_table_words(n_tensors, n_peers) + n_peers /* shares */ + n_peers * kPeerBlocks) * 8;
+  return (peer_table_words(n_tensors, n_peers) + n_peers /* shares */ + n_peers * peer_blocks(static_cast<int>(n_peers))) * 8;
 }
 
 struct Round {  // a round's arguments, as the entry points give them
@@ -984,15 +998,19 @@ struct Round {  // a round's arguments, as the entry points give them
 
 int check_round(const char* what, const Round& r, std::vector<int>* order) {
   const std::string w(what);
-  if (r.n_peers < 1 || r.n_peers > kMostPeers) return fail(DLA_E_INVALID, w + ": n_peers must be 1.." + std::to_string(kMostPeers));
+  if (r.n_peers < 1 || r.n_peers > kMostPeers)
+    return fail(DLA_E_INVALID, w + ": n_peers must be 1.." + std::to_string(kMostPeers));
   if (r.n_tensors < 0) return fail(DLA_E_INVALID, w + ": n_tensors < 0");
   if (r.n_tensors > 0 && (!r.dtypes || !r.peers || !r.centers || !r.numels)) return fail(DLA_E_INVALID, w + ": null array");
   for (int t = 0; t < r.n_tensors; ++t) {
-    if (!known_dtype(r.dtypes[t])) return fail(DLA_E_INVALID, w + ": tensor " + std::to_string(t) + " has unknown dtype " + std::to_string(r.dtypes[t]));
-    if (r.numels[t] < 0 || r.numels[t] > kMostElems) return fail(DLA_E_INVALID, w + ": tensor " + std::to_string(t) + " has a bad element count");
+    if (!known_dtype(r.dtypes[t]))
+      return fail(DLA_E_INVALID, w + ": tensor " + std::to_string(t) + " has unknown dtype " + std::to_string(r.dtypes[t]));
+    if (r.numels[t] < 0 || r.numels[t] > kMostElems)
+      return fail(DLA_E_INVALID, w + ": tensor " + std::to_string(t) + " has a bad element count");
     if (r.numels[t] == 0) continue;
     const int es = elem_bytes(r.dtypes[t]);
-    if (!r.centers[t] || !aligned_to(r.centers[t], es)) return fail(DLA_E_INVALID, w + ": centre tensor " + std::to_string(t) + " is null or not aligned");
+    if (!r.centers[t] || !aligned_to(r.centers[t], es))
+      return fail(DLA_E_INVALID, w + ": centre tensor " + std::to_string(t) + " is null or not aligned");
     for (int k = 0; k < r.n_peers; ++k) {
       const void* p = r.peers[static_cast<int64_t>(t) * r.n_peers + k];
       if (!p || !aligned_to(p, es))
@@ -1006,7 +1024,8 @@ int check_round(const char* what, const Round& r, std::vector<int>* order) {
   std::vector<Span> spans;
   for (int t : *order) {
     const int es = elem_bytes(r.dtypes[t]);
-    if (!r.outs[t] || !aligned_to(r.outs[t], es)) return fail(DLA_E_INVALID, w + ": out " + std::to_string(t) + " is null or not aligned");
+    if (!r.outs[t] || !aligned_to(r.outs[t], es))
+      return fail(DLA_E_INVALID, w + ": out " + std::to_string(t) + " is null or not aligned");
     spans.push_back(span_of(r.outs[t], r.numels[t], es));
   }
   const std::vector<Span> own = spans;
@@ -1027,6 +1046,14 @@ int64_t units_of(int64_t n, int dt, int unit_bytes) {
   return (n + per - 1) / per;
 }
 
+// Page-locked memory that kernels reach at the same address?
+bool mapped_host(const void* p) {
+  hipPointerAttribute_t a;
+  const bool ok = hipPointerGetAttributes(&a, p) == hipSuccess && a.type == hipMemoryTypeHost && a.devicePointer == p;
+  if (!ok) (void)hipGetLastError();
+  return ok;
+}
+
 // The round's table: in `words` if it fits there, else in the workspace.
 int make_table(const char* what, const Round& r, const std::vector<int>& order, int norm_unit, void* table_host,
                int64_t table_host_bytes, uint64_t* workspace, PutWords* words, Table* tab, int64_t* norm_units,
@@ -1034,7 +1061,7 @@ int make_table(const char* what, const Round& r, const std::vector<int>& order, 
   const int m = static_cast<int>(order.size());
   const int64_t n_words = peer_table_words(m, r.n_peers);
   const bool here = n_words <= kPutWords;
-  const bool host = !here && table_host && table_host_bytes >= n_words * 8 && aligned_to(table_host, 8);
+  const bool host = !here && table_host && table_host_bytes >= n_words * 8 && aligned_to(table_host, 8) && mapped_host(table_host);
   std::vector<uint64_t> built(here || host ? 0 : static_cast<size_t>(n_words));
   uint64_t* to = here ? words->w : host ? static_cast<uint64_t*>(table_host) : built.data();
   Seg* segs = reinterpret_cast<Seg*>(to);
@@ -1070,7 +1097,7 @@ int make_table(const char* what, const Round& r, const std::vector<int>& order, 
 struct NormLaunch {
   const PutWords& words;
   Table tab;
-  bool tiled, wide;  // wide: kPeerVec loads of one peer in a row
+  bool tiled;
   dim3 grid;
   hipStream_t s;
   int64_t units;
@@ -1079,16 +1106,12 @@ struct NormLaunch {
   uint32_t* counters;
   const Joined& to;
 };
-template <int G, int V, bool TILED>
-void launch_peer_norms(const NormLaunch& a) {
-  hipLaunchKernelGGL((peer_norms_kernel<G, V, TILED>), a.grid, dim3(kThreads), 0, a.s, a.words, a.tab, a.units, a.l, a.partials,
-                     a.counters, a.to);
-}
 template <int G>
 void launch_peer_norms(const NormLaunch& a) {
-  if (a.tiled) launch_peer_norms<G, 1, true>(a);
-  else if (a.wide) launch_peer_norms<G, kPeerVec, false>(a);
-  else launch_peer_norms<G, 1, false>(a);
+  if (a.tiled)
+    hipLaunchKernelGGL((peer_norms_kernel<G, true>), a.grid, dim3(kThreads), 0, a.s, a.words, a.tab, a.units, a.l, a.partials, a.counters, a.to);
+  else
+    hipLaunchKernelGGL((peer_norms_kernel<G, false>), a.grid, dim3(kThreads), 0, a.s, a.words, a.tab, a.units, a.l, a.partials, a.counters, a.to);
 }
 
 // The norms (no sq_in), then the average (outs != null), of one round.
@@ -1100,6 +1123,7 @@ int round_impl(const char* what, const Round& r, double max_norm, const double* 
   const std::string w(what);
   if (norms && ((out_dtype != DLA_F32 && out_dtype != DLA_F64) || !aligned_to(norms, elem_bytes(out_dtype))))
     return fail(DLA_E_INVALID, w + ": norms must be aligned F32 or F64 values");
+  if (!aligned_to(sq_in, 8) || !aligned_to(sq_out, 8)) return fail(DLA_E_INVALID, w + ": squared norms are not aligned");
   if (!aligned_to(counters, 4)) return fail(DLA_E_INVALID, w + ": counters are not aligned");
   if (r.outs && !r.weights) return fail(DLA_E_INVALID, w + ": null weights");
   if (r.outs && !(max_norm >= 0)) return fail(DLA_E_INVALID, w + ": max_norm must be >= 0");
@@ -1108,11 +1132,10 @@ int round_impl(const char* what, const Round& r, double max_norm, const double* 
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int m = static_cast<int>(order.size()), n = r.n_peers;
   uint64_t* table = static_cast<uint64_t*>(workspace);
-  const bool wide = !r.tiled;
   int64_t norm_units = 0, mean_units = 0;
   PutWords words;
   Table tab;
-  if (int rc = make_table(what, r, order, wide ? kNormUnit * kPeerVec : kNormUnit, table_host, table_host_bytes, table, &words,
+  if (int rc = make_table(what, r, order, unit_bytes(peer_vec(r.tiled)), table_host, table_host_bytes, table, &words,
                           &tab, &norm_units, &mean_units, s))
     return rc;
   double* shares = reinterpret_cast<double*>(table + peer_table_words(r.n_tensors, n));
@@ -1120,16 +1143,12 @@ int round_impl(const char* what, const Round& r, double max_norm, const double* 
   const Joined to = {sq_in, sq_out, norms, out_dtype, r.outs ? shares : nullptr, max_norm};
   int64_t blocks = 0;
   if (!sq_in && m > 0) {
-    // peers beside one read of the centre: 8 at most (their loads are all in flight), groups of equal size
-    const int groups = (n + 7) / 8, g = (n + groups - 1) / groups;
-    // from 5 groups on, as many workgroups as run at once (2 per CU): 128 x 21.3 M bf16 852 us, 871 with twice as
-    // many; with fewer groups the second half evens out the first (16 x ResNet-34 bf16 127, 131 with half)
-    const int most = groups > 4 ? kPeerBlocks / 2 : kPeerBlocks;
-    blocks = std::min<int64_t>(norm_units, std::max<int64_t>(1, most / groups));
+    const int groups = peer_groups(n), g = (n + groups - 1) / groups;
+    blocks = std::min(norm_units, peer_blocks(n));
     // large rounds join in a kernel of its own: its launch hides behind the round, the last workgroup's join does
     // not (us, apart / in the last workgroup: 8 x 25 M f32 138.6 / 141.6; but 2 x 85 K f32 with the average 15.5 / 12.7)
-    if (blocks * groups > kPeerBlocks / 2) counters = nullptr;
-    const NormLaunch a = {words, tab, r.tiled, wide, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>((n + g - 1) / g)), s,
+    if (blocks * groups > 512) counters = nullptr;
+    const NormLaunch a = {words, tab, r.tiled, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>((n + g - 1) / g)), s,
                           norm_units, r.layout, partials, static_cast<uint32_t*>(counters), to};
     switch (g) {
       case 1: launch_peer_norms<1>(a); break;
@@ -1155,10 +1174,11 @@ int round_impl(const char* what, const Round& r, double max_norm, const double* 
   // 14 waves per CU, by reserving LDS that nothing reads (us, 14 / uncapped: 8 x 25 M f32 157 / 165, 16 x ResNet-34
   // bf16 128.7 / 130.9, 128 x 2.7 M bf16 127.7 / 130.3); fewer peers lose by it (2 x 25 M f32 74 / 65), smaller
   // rounds tie (32 x 1.7 M f32 43.3 / 43.0).
-  int64_t bytes = 0;
-  for (int t : order) bytes += r.numels[t] * elem_bytes(r.dtypes[t]) * (n + 1);
-  const int lds = n >= 8 && bytes > (int64_t{256} << 20) ? 160 * 1024 / 14 : 0;
-  if (r.tiled) hipLaunchKernelGGL((bounded_kernel<true>), grid, dim3(kMeanThreads), lds, s, words, tab, mean_units, shares, r.layout);
+  double bytes = 0;
+  for (int t : order) bytes += static_cast<double>(r.numels[t]) * elem_bytes(r.dtypes[t]) * (n + 1);
+  const int lds = n >= 8 && bytes > kInfinityCache ? 160 * 1024 / 14 : 0;
+  if (r.tiled)
+    hipLaunchKernelGGL((bounded_kernel<true>), grid, dim3(kMeanThreads), lds, s, words, tab, mean_units, shares, r.layout);
   else hipLaunchKernelGGL((bounded_kernel<false>), grid, dim3(kMeanThreads), lds, s, words, tab, mean_units, shares, r.layout);
   if (hipError_t e = hipGetLastError()) return hip_fail(what, e);
   return DLA_OK;
@@ -1179,9 +1199,12 @@ int slab_round(const char* what, SlabRound* sr, int dtype, const void* base, int
   if (!known_dtype(dtype)) return fail(DLA_E_INVALID, w + ": unknown dtype " + std::to_string(dtype));
   if (n_elems < 0 || n_elems > kMostElems) return fail(DLA_E_INVALID, w + ": bad element count");
   const int es = elem_bytes(dtype);
-  if (!base || !aligned_to(base, 16) || tile_elems * es < 16 || tile_elems > (int64_t{1} << 40) || (tile_elems & (tile_elems - 1)))
+  if (!base || !aligned_to(base, 16) || tile_elems < 1 || tile_elems > (int64_t{1} << 30) || tile_elems * es < 16 || (tile_elems & (tile_elems - 1)))
     return fail(DLA_E_INVALID, w + ": base must be 16-byte aligned and tile_elems a power of two of >= 16 bytes");
-  if (n_peers < 1 || n_peers > kMostPeers || slab_rows < n_peers) return fail(DLA_E_INVALID, w + ": need 1 <= n_peers <= slab_rows and n_peers <= " + std::to_string(kMostPeers));
+  if (static_cast<double>(n_elems + tile_elems) * es * static_cast<double>(slab_rows) > static_cast<double>(kMostElems))
+    return fail(DLA_E_INVALID, w + ": slab_rows x n_elems is beyond any device");
+  if (n_peers < 1 || n_peers > kMostPeers || slab_rows < n_peers)
+    return fail(DLA_E_INVALID, w + ": need 1 <= n_peers <= slab_rows and n_peers <= " + std::to_string(kMostPeers));
   int shift = 0;
   while ((int64_t{1} << shift) < tile_elems) ++shift;
   sr->dtype = dtype;
@@ -1208,6 +1231,8 @@ int guarded(const char* what, F f) {
   dla_internal_clear_error();
   try {
     return f();
+  } catch (const std::bad_alloc&) {
+    return dla_internal_fail(DLA_E_INVALID, "no memory");
   } catch (const std::exception& e) {
     return fail(DLA_E_INVALID, std::string(what) + ": " + e.what());
   } catch (...) {
@@ -1256,7 +1281,8 @@ int dla_peer_norms(int n_tensors, const int* dtypes, const void* const* peer_ptr
                    void* table_host, int64_t table_host_bytes, void* workspace, int64_t workspace_bytes, void* stream) {
   return guarded("dla_peer_norms", [&] {
     const Round r = {n_tensors, dtypes, peer_ptrs, centers, nullptr, numels, nullptr, n_peers, {0, 0, 0}, false};
-    return round_impl("dla_peer_norms", r, 0, nullptr, sq_out, out_dtype, norms, counters, table_host, table_host_bytes, workspace, workspace_bytes, stream);
+    return round_impl("dla_peer_norms", r, 0, nullptr, sq_out, out_dtype, norms, counters, table_host,
+                      table_host_bytes, workspace, workspace_bytes, stream);
   });
 }
 
@@ -1268,7 +1294,8 @@ int dla_wsum_bounded(int n_tensors, const int* dtypes, const void* const* peer_p
     if (!outs && n_tensors > 0) return fail(DLA_E_INVALID, "dla_wsum_bounded: null outs array");
     static void* const none[1] = {nullptr};
     const Round r = {n_tensors, dtypes, peer_ptrs, centers, outs ? outs : none, numels, weights, n_peers, {0, 0, 0}, false};
-    return round_impl("dla_wsum_bounded", r, max_norm, sq, nullptr, out_dtype, norms, counters, table_host, table_host_bytes, workspace, workspace_bytes, stream);
+    return round_impl("dla_wsum_bounded", r, max_norm, sq, nullptr, out_dtype, norms, counters, table_host,
+                      table_host_bytes, workspace, workspace_bytes, stream);
   });
 }
 
@@ -1279,8 +1306,10 @@ int dla_wsum_bounded_slab_tiled(int dtype, const void* base, int64_t tile_elems,
   return guarded("dla_wsum_bounded_slab_tiled", [&] {
     if (!out && n_elems > 0) return fail(DLA_E_INVALID, "dla_wsum_bounded_slab_tiled: null out");
     SlabRound sr;
-    if (int rc = slab_round("dla_wsum_bounded_slab_tiled", &sr, dtype, base, tile_elems, slab_rows, center, n_peers, n_elems, out, weights)) return rc;
-    return round_impl("dla_wsum_bounded_slab_tiled", sr.r, max_norm, nullptr, nullptr, out_dtype, norms, counters, nullptr, 0, workspace, workspace_bytes, stream);
+    if (int rc = slab_round("dla_wsum_bounded_slab_tiled", &sr, dtype, base, tile_elems, slab_rows, center, n_peers, n_elems, out, weights))
+      return rc;
+    return round_impl("dla_wsum_bounded_slab_tiled", sr.r, max_norm, nullptr, nullptr, out_dtype, norms, counters,
+                      nullptr, 0, workspace, workspace_bytes, stream);
   });
 }
 

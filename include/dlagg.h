@@ -250,7 +250,7 @@ int64_t dla_norm_workspace(int n_tensors);
 int dla_norm(int n_tensors, const int* dtypes, const void* const* tensors, const int64_t* numels, int norm, int out_dtype,
              void* out, void* counter, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* outs[t] = round(tensors[t] * min(1, max_norm / (n + eps))), n the norm of the tensors.  NaN norms make everything NaN,
+/* outs[t] = round(tensors[t] * min(1, max_norm / (n + eps))), n the norm of the tensors, eps > 0.  NaN norms make everything NaN,
  * infinite ones give a factor of 0.  outs[t] may be tensors[t]; every other overlap is refused (DLA_E_ALIAS).  In
  * place nothing is written when the factor is 1.  norm_out (F32 or F64, DEVICE) may be NULL. */
 int dla_norm_clip(int n_tensors, const int* dtypes, const void* const* tensors, void* const* outs, const int64_t* numels,

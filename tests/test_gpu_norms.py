@@ -844,6 +844,49 @@ def test_counters_are_zero_again_and_calls_without_them_agree():
         assert all(torch.equal(a, b) for a, b in zip(eager[0], captured))
 
 
+def test_large_tables_captured_and_with_every_slot_taken():
+    """Tables beyond the launches' arguments: from page-locked memory, by value under capture, and by value when
+    other threads hold every slot of page-locked memory."""
+    from accdfl_amd.core import norms, wsum
+
+    sizes = [1 + i * 53 % 3000 for i in range(60)]
+    center, models, weights = _round(40, sizes, "bf16", seed=22)
+    outs = [torch.zeros_like(c) for c in center]
+    want, wn, added = no.bounded(models, weights, center, 0.5)
+
+    def check(norms_got):
+        torch.cuda.synchronize()
+        no.assert_norm(norms_got, wn, sum(sizes))
+        for o, w, a in zip(outs, want, added):
+            no.assert_close(o, w, sum(sizes), a)
+            o.zero_()
+
+    run = lambda: norms.wsum_bounded_multi(models, weights, center, 0.5, outs)  # noqa: E731
+    for _ in range(20):  # more calls than slots
+        got = run()
+    check(got)
+    ring = wsum.table_ring(torch.device("cuda", 0))
+    taken = [ring.take(8) for _ in range(ring.SLOTS)]
+    assert ring.take(8, wait=False) is None
+    check(run())
+    for idx, _, _ in taken:
+        ring.done(idx, torch.cuda.current_stream())
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        check(run())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        captured = run()
+    for _ in range(3):
+        run()
+        for o in outs:
+            o.zero_()
+        captured.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        check(captured)
+
+
 def test_error_if_nonfinite_is_refused_under_capture():
     from accdfl_amd.core.norms import clip_global_norm_
 

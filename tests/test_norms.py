@@ -83,6 +83,7 @@ def _clip(L, n=1, codes=None, ptrs=None, outs=None, numels=None, max_norm=1.0, e
     (dict(max_norm=-1.0), -1, "max_norm"),
     (dict(max_norm=math.nan), -1, "max_norm"),
     (dict(eps=-1.0), -1, "eps"),
+    (dict(eps=0.0), -1, "eps"),
     (dict(outs=_ptrs(None)), -1, "null"),
     (dict(outs=_ptrs(B + 1)), -1, "not aligned"),
     (dict(norm_out=0x40002), -1, "F32 or F64"),
@@ -101,10 +102,11 @@ def test_norm_clip_refusals(L, kw, rc_want, text):
 
 
 def _bounded(L, n=1, peers=2, codes=None, ptrs=None, centers=None, outs=None, numels=None, weights=True, max_norm=1.0,
-             norms=None, counters=None, ws=WS, nbytes=BIG):
+             norms=None, counters=None, ws=WS, nbytes=BIG, sq=None):
     return _err(L, L.so.dla_wsum_bounded(
         n, codes or _ints(0), ptrs or _ptrs(A, B), centers or _ptrs(0x30000), outs or _ptrs(0x40000), numels or _longs(4),
-        (ctypes.c_double * max(1, peers))(*[0.5] * max(1, peers)) if weights else None, peers, max_norm, None, 0, norms, counters,
+        (ctypes.c_double * max(1, peers))(*[0.5] * max(1, peers)) if weights else None, peers, max_norm,
+        ctypes.cast(sq, ctypes.POINTER(ctypes.c_double)) if sq else None, 0, norms, counters,
         None, 0, ws, nbytes, None))
 
 
@@ -123,6 +125,7 @@ def _bounded(L, n=1, peers=2, codes=None, ptrs=None, centers=None, outs=None, nu
     (dict(max_norm=math.nan), -1, "max_norm"),
     (dict(norms=0x50002), -1, "norms"),
     (dict(counters=0x50002), -1, "counters"),
+    (dict(sq=0x50004), -1, "squared norms"),
     (dict(ws=None), -1, "workspace"),
     (dict(nbytes=128), -1, "workspace"),
     (dict(outs=_ptrs(B + 4)), -2, "peer 1"),
@@ -144,6 +147,9 @@ def test_bounded_refusals(L, kw, rc_want, text):
     (dict(base=None), -1, "base"),
     (dict(base=A + 8), -1, "16-byte"),
     (dict(rows=1), -1, "slab_rows"),
+    (dict(rows=1 << 60), -1, "beyond any device"),
+    (dict(tile=0), -1, "power of two"),
+    (dict(tile=1 << 40), -1, "power of two"),
     (dict(n=0), -1, "n_peers"),
     (dict(numel=-1), -1, "element count"),
     (dict(out=None), -1, "null out"),
@@ -284,6 +290,18 @@ def _hip_bounded():
         out.copy_(norms.wsum_bounded([p.to(dev) for p in peers], weights, center.to(dev), max_norm,
                                      sq_norms=sq.to(dev))[0].cpu())
     return sq_norms, average
+
+
+def test_sharded_bound_is_checked_before_the_collective():
+    from accdfl_amd.core.sharding import BucketShardedFedAvg
+
+    def never(*_):
+        raise AssertionError("reached")
+
+    sh = BucketShardedFedAvg(64, torch.float32, device=torch.device("cpu"), bounded=(never, never))
+    for bad in (-1.0, math.nan):
+        with pytest.raises(ValueError, match="max_norm"):
+            sh.reduce_bucket_bounded([torch.zeros(64)], torch.zeros(64), bad)
 
 
 def _sharded_inputs(n_peers, n_elems):
