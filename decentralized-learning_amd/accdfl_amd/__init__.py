@@ -10,6 +10,8 @@ Import layout mirrors the reference package:
     accdfl_amd.core.gradient_aggregation            <- accdfl/core/gradient_aggregation/__init__.py
     accdfl_amd.core.gradient_aggregation.fedavg     <- accdfl/core/gradient_aggregation/fedavg.py
     accdfl_amd.core.model_manager                   <- accdfl/core/model_manager.py (aggregation part)
+    accdfl_amd.core.gradient_aggregation.norm_bounded  FedAvg of updates bounded by their norms
+    accdfl_amd.core.norms                           norms over many tensors, clipped gradients, bounded averages
     accdfl_amd.core.peer_slab                       device staging of received peer models (HBM)
     accdfl_amd.core.sharding                        parameter-bucket sharding over ranks (RCCL)
 """

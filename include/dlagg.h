@@ -36,7 +36,8 @@
  * Surface.  The drop-in for the reference path is: dla_wsum, dla_wsum_multi(_table[_acc]),
  * dla_wsum_mixed, dla_wsum_slab(_tiled) + dla_slab_stage, dla_wsum_sharded, dla_host_round_start /
  * _finish, dla_host_reduce / dla_host_reduce_launch / _join, dla_plan_*, dla_mean and the helpers
- * (version, build id, last error, shard range, tile size, copy batch, shutdown).  INTERNAL entry
+ * (version, build id, last error, shard range, tile size, copy batch, shutdown).  Beyond the
+ * reference: dla_norm(_clip), dla_peer_norms and dla_wsum_bounded(_slab_tiled).  INTERNAL entry
  * points — exported for the library's own tests, benchmarks and diagnostics, not part of the
  * drop-in and free to change: dla_wsum_ex (forced launch knobs), dla_select_kernel,
  * dla_host_in_place_rounds, dla_host_reduce_deferred (dla_host_reduce_launch's body on the
@@ -227,8 +228,8 @@ int dla_mean(int dtype, const void* const* peers, int n_peers, int64_t n_elems, 
 /* ---- norms over many tensors, and what is bounded by them (additive in ABI v13) ----
  *
  * Tensors are dense and of any of the four dtypes, mixed freely within a call; their pointers need element
- * alignment only.  The sums of norms are carried in 64 bits.  Nothing synchronises; the stream's device must be
- * current.  Without a table_host, launches take everything by value except the caller's buffers, so a captured call
+ * alignment only.  The sums of norms are carried in 64 bits (F64 elements beyond 1e154 make an infinite norm).
+ * Nothing synchronises; the stream's device must be current.  Without a table_host, launches take everything by value except the caller's buffers, so a captured call
  * replays.  The workspaces are the caller's, need no initialisation and hold nothing between calls; two calls in
  * flight at once need two.  The counters (NULL: one launch more) let a kernel's last workgroup add up what the others
  * found: DEVICE memory, DLA_COUNTER_BYTES zero bytes, which are zero again when the call's work is done; calls on one
@@ -250,9 +251,9 @@ int64_t dla_norm_workspace(int n_tensors);
 int dla_norm(int n_tensors, const int* dtypes, const void* const* tensors, const int64_t* numels, int norm, int out_dtype,
              void* out, void* counter, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* outs[t] = round(tensors[t] * min(1, max_norm / (n + eps))), n the norm of the tensors, eps > 0.  NaN norms make everything NaN,
- * infinite ones give a factor of 0.  outs[t] may be tensors[t]; every other overlap is refused (DLA_E_ALIAS).  In
- * place nothing is written when the factor is 1.  norm_out (F32 or F64, DEVICE) may be NULL. */
+/* outs[t] = round(tensors[t] * min(1, max_norm / (n + eps))), n the norm of the tensors, eps > 0.  NaN norms make
+ * everything NaN, infinite ones give a factor of 0.  outs[t] may be tensors[t]; every other overlap is refused
+ * (DLA_E_ALIAS).  In place nothing is written when the factor is 1.  norm_out (F32 or F64, DEVICE) may be NULL. */
 int dla_norm_clip(int n_tensors, const int* dtypes, const void* const* tensors, void* const* outs, const int64_t* numels,
                   int norm, double max_norm, double eps, int out_dtype, void* norm_out, void* counter, void* workspace,
                   int64_t workspace_bytes, void* stream);
@@ -279,8 +280,8 @@ int dla_peer_norms(int n_tensors, const int* dtypes, const void* const* peer_ptr
 /* fedavg.py:20-25 with every peer's update bounded first:
  *     out = round(c + sum_k a_k (p_k - c)),   a_k = weights[k] * (n_k <= max_norm ? 1 : max_norm / n_k)
  * with n_k as dla_peer_norms gives it, in list order, carried in 64 bits (32 for BF16 and F16) and rounded once
- * (dla_wsum rounds every step, as the reference does).  A peer whose n_k is not finite adds nothing and is not read.  outs[t] may be
- * tensor t of the centre or of a peer; every other overlap is refused (DLA_E_ALIAS).
+ * (dla_wsum rounds every step, as the reference does).  A peer whose n_k is not finite adds nothing and is not
+ * read.  outs[t] may be tensor t of the centre or of a peer; every other overlap is refused (DLA_E_ALIAS).
  *   sq  DEVICE doubles [n_peers], the squared norms to bound by (a bucket of a model whose norms are known), or
  *       NULL: computed here */
 int dla_wsum_bounded(int n_tensors, const int* dtypes, const void* const* peer_ptrs, const void* const* centers,
