@@ -742,7 +742,8 @@ __global__ __launch_bounds__(kMeanThreads) void bounded_kernel(const PutWords wo
 // ------------------------------------------------------------------ host side
 int fail(int code, const std::string& msg) { return dla_internal_fail(code, msg.c_str()); }
 int hip_fail(const char* what, hipError_t e) {
-  return fail(static_cast<int>(e), std::string(what) + ": " + hipGetErrorString(e)); }
+  return fail(static_cast<int>(e), std::string(what) + ": " + hipGetErrorString(e));
+}
 
 bool known_dtype(int dt) { return dt == DLA_F32 || dt == DLA_BF16 || dt == DLA_F16 || dt == DLA_F64; }
 bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
