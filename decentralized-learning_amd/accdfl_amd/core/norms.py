@@ -105,6 +105,14 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _held(t: torch.Tensor) -> bool:
+    """The tensor's storage holds every one of its elements (one that was resized under it may not)."""
+    if t.numel() == 0:
+        return True
+    last = t.storage_offset() + sum((size - 1) * stride for size, stride in zip(t.shape, t.stride()))
+    return t.untyped_storage().nbytes() >= (last + 1) * t.element_size()
+
+
 def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.stride() == b.stride() or (a.is_contiguous() and b.is_contiguous())
 
@@ -127,6 +135,8 @@ def _check(lists: List[List[torch.Tensor]], names: Sequence[str]) -> torch.devic
                 device = _wsum.require_device(t.device if t.is_cuda else None)
             if t.device != device:
                 raise ValueError("%s is on %s, expected %s" % (what, t.device, device))
+            if not _held(t):
+                raise ValueError("%s lies outside its storage (%d bytes)" % (what, t.untyped_storage().nbytes()))
             if t.dtype != first[i].dtype or t.shape != first[i].shape:
                 raise ValueError("%s is %s %s, %s has %s %s there" % (what, t.dtype, tuple(t.shape), names[0],
                                                                       first[i].dtype, tuple(first[i].shape)))

@@ -346,8 +346,9 @@ std::unique_ptr<DenseTables> pack_lists(const std::vector<std::vector<PyObject*>
       if (!THPVariable_Check(o)) return nullptr;
       const at::Tensor& x = THPVariable_Unpack(o);
       if (x.layout() != at::kStrided || !x.is_cuda() || x.is_neg() || x.unsafeGetTensorImpl()->is_python_dispatch() ||
-          !x.is_non_overlapping_and_dense())
-        return nullptr;
+          !x.is_non_overlapping_and_dense() || !x.has_storage() ||
+          x.storage().nbytes() < static_cast<size_t>((x.storage_offset() + x.numel()) * x.element_size()))
+        return nullptr;  // the last: a storage that was resized under the tensor
       if (device < 0) device = x.get_device();
       if (x.get_device() != device) return nullptr;
       int32_t code;

@@ -887,6 +887,24 @@ def test_large_tables_captured_and_with_every_slot_taken():
         check(captured)
 
 
+def test_released_storages_are_refused():
+    from accdfl_amd.core import norms
+
+    kept, freed = torch.ones(64, device="cuda"), torch.ones(64, device="cuda")
+    part = freed[16:32]
+    freed.untyped_storage().resize_(0)
+    for bad in (freed, part):
+        with pytest.raises(ValueError, match="outside its storage"):
+            norms.global_norm([kept, bad])
+        with pytest.raises(ValueError, match="outside its storage"):
+            norms.clip_global_norm_([kept, bad], 1.0)
+        with pytest.raises(ValueError, match="outside its storage"):
+            norms.update_norms([[bad]], [torch.zeros(bad.shape, device="cuda")])
+        with pytest.raises(ValueError, match="outside its storage"):
+            norms.wsum_bounded([torch.zeros(bad.shape, device="cuda")], [1.0], bad, 1.0)
+    assert norms.global_norm([kept]).item() == 8.0
+
+
 def test_error_if_nonfinite_is_refused_under_capture():
     from accdfl_amd.core.norms import clip_global_norm_
 

@@ -292,6 +292,18 @@ def _hip_bounded():
     return sq_norms, average
 
 
+def test_tensors_outside_their_storage_are_seen():
+    from accdfl_amd.core.norms import _held
+
+    base = torch.zeros(100)
+    views = [base, base[40:60], base[::7], base.view(10, 10).t(), base[3:4].expand(5), base[:0]]
+    assert all(_held(v) for v in views)
+    base.untyped_storage().resize_(4 * 70)
+    assert [_held(v) for v in views] == [False, True, False, False, True, True]
+    base.untyped_storage().resize_(0)
+    assert [_held(v) for v in views] == [False] * 5 + [True]
+
+
 def test_sharded_bound_is_checked_before_the_collective():
     from accdfl_amd.core.sharding import BucketShardedFedAvg
 
