@@ -16,11 +16,11 @@ of a model once before the first element can be written, which is what these ope
 Tensors are float32 / bfloat16 / float16 / float64, mixed freely within a list, on one HIP device, empty ones
 included.  Dense tensors are read where they are whatever the order of their axes and wherever they start; others
 (a slice with gaps, an expanded tensor) are copied first.  Norms and products are carried in 64 bits, averages in 64
-(32 for the 16-bit types), and rounded once.  Results are on the device and nothing synchronises; nothing here is
-differentiable.  Work is enqueued on ``stream`` or the current stream of the tensors' device, workspaces come from
-torch's caching allocator for each call, and launches take their tables by value (those of large rounds from a slot
-of page-locked memory that the call owns until the GPU has read it; under capture by value too): calls on several
-streams or threads do not meet, and a call captured into a graph replays.
+(32 for the 16-bit types, where they hold every term), and rounded once.  Results are on the device and nothing
+synchronises; nothing here is differentiable.  Work is enqueued on ``stream`` or the current stream of the tensors'
+device, workspaces come from torch's caching allocator for each call, and launches take their tables by value (those
+of large rounds from a slot of page-locked memory that the call owns until the GPU has read it; under capture by value
+too): calls on several streams or threads do not meet, and a call captured into a graph replays.
 """
 from __future__ import annotations
 
@@ -432,9 +432,9 @@ def wsum_bounded_multi(peer_params: Sequence[Tensors], weights: Sequence[float],
         n_k     = || peer_k - center ||_2  over all its tensors
         outs[i] = center[i] + sum_k weights[k] * min(1, max_norm / n_k) * (peer_k[i] - center[i])
 
-    in list order, carried in 64 bits (32 for the 16-bit types) and rounded once.  A peer whose update is not
-    finite (n_k is NaN or infinite) adds nothing.  ``outs[i]`` may be the i-th tensor of the centre or of a peer; no
-    other overlap.  ``sq_norms``: float64 squared norms [n] on the device to bound by, when the tensors are one
+    in list order, carried in 64 bits (32 for the 16-bit types, where they hold every term) and rounded once.  A peer
+    whose update is not finite (n_k is NaN or infinite) adds nothing.  ``outs[i]`` may be the i-th tensor of the centre
+    or of a peer; no other overlap.  ``sq_norms``: float64 squared norms [n] on the device to bound by, when the tensors are one
     bucket of models whose norms are known (update_norms(squared=True), added up).  At most 2 048 peers.  Returns
     the norms [n], float32 (float64 if any tensor is)."""
     bound = _bound(max_norm)

@@ -12,7 +12,7 @@
 // Norms and products are carried in 64 bits whatever the storage type: a vector FMA in f64 issues at the
 // rate of one in f32 on this chip, the kernels wait for memory either way, and the square of any f32 value
 // is a normal f64, so no norm of finite 32- or 16-bit values overflows or underflows.  So are averages, but
-// for the 16-bit types (Average below).  A result is rounded to its storage type once (16-bit types through
+// for most of the 16-bit types (Average below).  A result is rounded to its storage type once (16-bit types through
 // f32: the first rounding moves a result by at most 2^-24 of itself).
 //
 // Work is cut into units of 1 to 32 KiB of one tensor; a unit never spans tensors.  The norms deal them round
@@ -143,28 +143,33 @@ template <> struct Elem<DLA_F16> {
   }
 };
 
-// The average's arithmetic: out = c + sum_k a_k (x_k - c).  In 64 bits for F32 and F64.  16-bit types, whose
-// result keeps 8 or 11 bits, take 32: half the registers and no conversions (us, 32 / 64 bits: 16 x ResNet-34 bf16
-// 130.5 / 136.1, 8 x 21.3 M f16 69.6 / 72.9, 128 x 21.3 M bf16 869 / 882).  There
-// the difference is taken of halves, one fma (x / 2 - c / 2) with the 2 in the share, so that two values at
-// opposite ends of bf16's range do not overflow it.
-template <int DT>
-struct Average {
+// The average's arithmetic: out = c + sum_k a_k (x_k - c), with a_k, the differences and the sum in `real`.  F32 and F64
+// take 64 bits.  16-bit types, whose result keeps 8 or 11 bits, take 32 where those hold every term (share32): half the
+// registers and no conversions (us, 32 bits / 32 and then 64: 16 x ResNet-34 bf16 130 / 278, 4 x 21.3 M bf16 43 / 66).
+struct Average64 {
   using real = double;
-  static __device__ inline double share(double a) { return a; }
-  static __device__ inline double center(double c) { return c; }
-  static __device__ inline double update(double x, double c) { return x - c; }
-  static __device__ inline double fold(double a, double d, double acc) { return __builtin_fma(a, d, acc); }
+  static __device__ inline const double* shares_of(const double* shares, int) { return shares; }
+  static __device__ inline double fold(double a, double x, double c, double acc) { return __builtin_fma(a, x - c, acc); }
 };
-struct Average16 {
+struct Average32 {
   using real = float;
-  static __device__ inline float share(double a) { return static_cast<float>(2.0 * a); }
-  static __device__ inline float center(float c) { return -0.5f * c; }
-  static __device__ inline float update(float x, float c) { return __builtin_fmaf(0.5f, x, c); }
-  static __device__ inline float fold(float a, float d, float acc) { return __builtin_fmaf(a, d, acc); }
+  static __device__ inline const float* shares_of(const double* shares, int n_peers) {  // behind those in 64 bits
+    return reinterpret_cast<const float*>(shares + n_peers);
+  }
+  static __device__ inline float fold(float a, float x, float c, float acc) { return __builtin_fmaf(a, x - c, acc); }
 };
-template <> struct Average<DLA_BF16> : Average16 {};
-template <> struct Average<DLA_F16> : Average16 {};
+template <int DT>
+using Average = std::conditional_t<DT == DLA_BF16 || DT == DLA_F16, Average32, Average64>;
+
+// a_k in 32 bits, NaN where 32 bits may not do: a peer's share below their normal range (it would lose bits, or count
+// for nothing), or differences, products or sums beyond it.  |x - c| <= n_k, so n_k <= 2^126 keeps differences in range
+// and |a_k| n_k <= 2^114 the sums over kMostPeers = 2^11 peers.  A NaN makes every sum of the round NaN, and what is NaN is
+// added up again in 64 bits (mean_unit): a round pays for its range only where it needs it.
+__device__ inline float share32(double share, double norm) {
+  const double a = __builtin_fabs(share);
+  const bool fits = a == 0.0 || (a >= 0x1p-126 && a <= 0x1p126 && norm <= 0x1p126 && a * norm <= 0x1p114);
+  return fits ? static_cast<float>(share) : __builtin_nanf("");
+}
 
 // Elements [j, j + n) of a tensor, n <= E: 16 bytes at once when n == E, else one by one with zeros behind.
 template <int DT>
@@ -576,6 +581,7 @@ struct Joined {
   void* norms;          // roots, of out_dt
   int out_dt;
   double* shares;       // a_k, by max_norm
+  float* shares32;      // share32 of them
   double max_norm;
 };
 // One wave: peer k's squared norm — the sum of its n partials (possibly none), or sq_in[k] — and what follows.
@@ -595,7 +601,9 @@ __device__ inline void join_peer(const double* partials, int n, int k, const dou
   if (to.norms) put_norm(to.norms, k, to.out_dt, norm);
   if (to.shares) {
     const double share = global_ptr<double>(weights)[k] * (norm <= to.max_norm ? 1.0 : to.max_norm / norm);
-    global_ptr<double>(to.shares)[k] = __builtin_isfinite(norm) ? share : 0.0;
+    const double counted = __builtin_isfinite(norm) ? share : 0.0;
+    global_ptr<double>(to.shares)[k] = counted;
+    global_ptr<float>(to.shares32)[k] = share32(counted, norm);
   }
 }
 
@@ -655,31 +663,57 @@ __global__ __launch_bounds__(64) void peer_join_kernel(const PutWords words, Tab
   join_peer(partials, n, static_cast<int>(blockIdx.x), parts_of(tab).weights, to);
 }
 
-template <int DT, int G, bool TILED>
-__device__ inline void fold_peers(const uint64_t* ptrs, const double* shares, const void* center, int64_t at, int64_t at_c,
-                                  bool full, int part, const typename Average<DT>::real (&c)[Elem<DT>::E],
-                                  typename Average<DT>::real (&acc)[Elem<DT>::E]) {
-  using A = Average<DT>;
+// G peers' terms, their loads all in flight.
+template <class A, int DT, int G, bool TILED>
+__device__ inline void fold_peers(const uint64_t* ptrs, const typename A::real* shares, const void* center, int64_t at,
+                                  int64_t at_c, bool full, int part, const typename A::real (&c)[Elem<DT>::E],
+                                  typename A::real (&acc)[Elem<DT>::E]) {
+  using R = typename A::real;
   constexpr int E = Elem<DT>::E;
   u32x4 r[G];
-  typename A::real a[G];
+  R a[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    const double share = const_ptr<double>(shares)[g];
+    a[g] = const_ptr<R>(shares)[g];
     const void* p = reinterpret_cast<const void*>(const_ptr<uint64_t>(ptrs)[g]);
-    const bool counts = share != 0.0;  // a peer that does not count is not read: the centre stands in, update 0
+    const bool counts = a[g] != R(0);  // a peer that does not count is not read: the centre stands in, update 0
     p = counts ? p : center;
     const int64_t from = TILED ? (counts ? at : at_c) : at;
-    a[g] = A::share(share);
     r[g] = full ? load_full<DT>(p, from) : load_part<DT>(p, from, part);
   }
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    typename A::real x[E];
+    R x[E];
     Elem<DT>::widen(r[g], x);
 #pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] = A::fold(a[g], A::update(x[i], c[i]), acc[i]);
+    for (int i = 0; i < E; ++i) acc[i] = A::fold(a[g], x[i], c[i], acc[i]);
   }
+}
+
+// Elements [j, j + part) of the average, G peers at a time and then what is left by halves.
+template <class A, int DT, int G, bool TILED>
+__device__ inline void average(const uint64_t* ptrs, const double* shares_of_all, int n_peers, const void* center, u32x4 rc,
+                               int64_t at, int64_t at_c, bool full, int part, typename A::real (&acc)[Elem<DT>::E]) {
+  constexpr int E = Elem<DT>::E;
+  const typename A::real* shares = A::shares_of(shares_of_all, n_peers);
+  typename A::real c[E];
+  Elem<DT>::widen(rc, c);
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0;
+  int i = 0;
+  for (; i + G <= n_peers; i += G) fold_peers<A, DT, G, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
+  if (G > 4 && i + 4 <= n_peers) {
+    fold_peers<A, DT, 4, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
+    i += 4;
+  }
+  if (G > 2 && i + 2 <= n_peers) {
+    fold_peers<A, DT, 2, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
+    i += 2;
+  }
+  if (G > 1 && i < n_peers) fold_peers<A, DT, 1, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
+  // where the centre is not finite no peer counts, and the centre stays
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = __builtin_isfinite(c[e]) ? acc[e] + c[e] : c[e];
 }
 
 template <int DT, bool TILED>
@@ -692,26 +726,22 @@ __device__ inline void mean_unit(const Layout& l, const uint64_t* ptrs, const do
   const bool full = (unit + 1) * (kMeanThreads * E) <= n;
   const int part = full ? E : clamp_part(n - j, E);
   const u32x4 rc = full ? load_full<DT>(center, at_c) : load_part<DT>(center, at_c, part);
-  typename A::real c[E], acc[E] = {};
-  Elem<DT>::widen(rc, c);
+  typename A::real acc[E];
+  average<A, DT, 8, TILED>(ptrs, shares, n_peers, center, rc, at, at_c, full, part, acc);
+  u32x4 mean = Elem<DT>::narrow(acc);
+  if constexpr (std::is_same_v<A, Average32>) {
+    // NaN: a share that 32 bits do not hold, or the data's own, which stays one.  Nothing is written yet, so the output
+    // may be an input here too; one peer at a time, for the registers.
+    bool again = false;
 #pragma unroll
-  for (int e = 0; e < E; ++e) c[e] = A::center(c[e]);
-  int i = 0;
-  for (; i + 8 <= n_peers; i += 8) fold_peers<DT, 8, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
-  if (i + 4 <= n_peers) {
-    fold_peers<DT, 4, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
-    i += 4;
+    for (int e = 0; e < E; ++e) again |= acc[e] != acc[e];
+    if (again) {
+      double wide[E];
+      average<Average64, DT, 1, TILED>(ptrs, shares, n_peers, center, rc, at, at_c, full, part, wide);
+      mean = Elem<DT>::narrow(wide);
+    }
   }
-  if (i + 2 <= n_peers) {
-    fold_peers<DT, 2, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
-    i += 2;
-  }
-  if (i < n_peers) fold_peers<DT, 1, TILED>(ptrs + i, shares + i, center, at, at_c, full, part, c, acc);
-  Elem<DT>::widen(rc, c);
-  // where the centre is not finite no peer counts, and the centre stays
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = __builtin_isfinite(c[e]) ? acc[e] + c[e] : c[e];
-  store_part<DT>(out, j, part, Elem<DT>::narrow(acc));
+  store_part<DT>(out, j, part, mean);
 }
 
 // out = round(c + sum_k a_k (p_k - c)).  Units are dealt from the last to the first: what the norms read last is
@@ -980,8 +1010,9 @@ int64_t peer_blocks(int n) {
 int64_t peer_table_words(int64_t n_tensors, int64_t n_peers) {
   return n_tensors * static_cast<int64_t>(sizeof(Seg) / 8) + n_tensors * n_peers + n_peers;
 }
+int64_t share_words(int64_t n_peers) { return n_peers + (n_peers + 1) / 2; }  // in 64 bits and in 32
 int64_t peer_workspace_bytes(int64_t n_tensors, int64_t n_peers) {
-  return (peer_table_words(n_tensors, n_peers) + n_peers /* shares */ + n_peers * peer_blocks(static_cast<int>(n_peers))) * 8;
+  return (peer_table_words(n_tensors, n_peers) + share_words(n_peers) + n_peers * peer_blocks(static_cast<int>(n_peers))) * 8;
 }
 
 struct Round {  // a round's arguments, as the entry points give them
@@ -1140,8 +1171,8 @@ int round_impl(const char* what, const Round& r, double max_norm, const double* 
                           &tab, &norm_units, &mean_units, s))
     return rc;
   double* shares = reinterpret_cast<double*>(table + peer_table_words(r.n_tensors, n));
-  double* partials = shares + n;
-  const Joined to = {sq_in, sq_out, norms, out_dtype, r.outs ? shares : nullptr, max_norm};
+  double* partials = shares + share_words(n);
+  const Joined to = {sq_in, sq_out, norms, out_dtype, r.outs ? shares : nullptr, reinterpret_cast<float*>(shares + n), max_norm};
   int64_t blocks = 0;
   if (!sq_in && m > 0) {
     const int groups = peer_groups(n), g = (n + groups - 1) / groups;

@@ -279,9 +279,9 @@ int dla_peer_norms(int n_tensors, const int* dtypes, const void* const* peer_ptr
 
 /* fedavg.py:20-25 with every peer's update bounded first:
  *     out = round(c + sum_k a_k (p_k - c)),   a_k = weights[k] * (n_k <= max_norm ? 1 : max_norm / n_k)
- * with n_k as dla_peer_norms gives it, in list order, carried in 64 bits (32 for BF16 and F16) and rounded once
- * (dla_wsum rounds every step, as the reference does).  A peer whose n_k is not finite adds nothing and is not
- * read.  outs[t] may be tensor t of the centre or of a peer; every other overlap is refused (DLA_E_ALIAS).
+ * with n_k as dla_peer_norms gives it, in list order, carried in 64 bits (for BF16 and F16 in 32, rounds with a share or a
+ * term beyond their normal range in 64) and rounded once (dla_wsum rounds every step, as the reference does).  A peer
+ * whose n_k is not finite adds nothing and is not read.  outs[t] may be tensor t of the centre or of a peer; every other overlap is refused (DLA_E_ALIAS).
  *   sq  DEVICE doubles [n_peers], the squared norms to bound by (a bucket of a model whose norms are known), or
  *       NULL: computed here */
 int dla_wsum_bounded(int n_tensors, const int* dtypes, const void* const* peer_ptrs, const void* const* centers,

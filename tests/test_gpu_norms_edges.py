@@ -1,0 +1,128 @@
+"""The norm operators at the ends of their ranges and of their contract: what a 16-bit average does with values and shares
+that float32 does not hold, which calls are refused, and what a refused call leaves as it was.  norms_oracle.py states the
+definitions and how far a correct result may be off.  Run on the MI355X: -m gpu."""
+import math
+
+import pytest
+import torch
+
+import norms_oracle as no
+from test_gpu_norms import DT, INF, _list, _native, _rand, _round  # noqa: F401 (the fixture is used by being here)
+
+pytestmark = pytest.mark.gpu
+
+
+def _row(values, dtype="bf16"):
+    return torch.tensor(values, dtype=torch.float64).to(DT[dtype]).cuda()
+
+
+def _assert_average(out, peers, weights, center, bound):
+    want, _, added = no.bounded([[p] for p in peers], weights, [center], bound)
+    no.assert_close(out, want[0], center.numel() + len(peers), added[0])
+
+
+# ------------------------------------------------------------------------- averages of 16-bit types in 64 bits
+# No term of these cases, or none before it is divided, lies in float32's normal range: the definition in 64 bits does.
+@pytest.mark.parametrize("peers, weights, center, bound", [
+    ([3e38], [1.0], -3e38, INF),
+    ([3e38, 3e38], [0.5, 0.5], -3e38, INF),
+    ([-3e38], [0.9], 1e38, INF),
+    ([3e38] * 130, [1.0 / 130] * 130, -3e38, INF),
+    ([3e38, 3e38, 3e38], [3.0, -2.5, 0.25], 0.0, INF),
+    ([1.0, 1.0, 1.0], [3e38, 3e38, -6e38], 0.0, INF),
+    ([1.0, 2.0], [1e-42, 3e-44], 0.0, INF),
+    ([3e38, 1.0], [1e-42, 1e-43], 1e-5, INF),
+    ([3e38, 0.5, 0.25], [1e-39, 0.25, 0.25], 0.0, INF),
+    ([1e20, -1e20], [1e30, 1e30], 0.0, INF),
+], ids=str)
+def test_bf16_averages_beyond_float32(peers, weights, center, bound):
+    from accdfl_amd.core.norms import wsum_bounded
+
+    for numel in (1, 7, 512, 1500):
+        c = torch.full((numel,), center, dtype=torch.bfloat16, device="cuda")
+        ps = [torch.full_like(c, p) for p in peers]
+        out, _ = wsum_bounded(ps, weights, c, bound)
+        _assert_average(out, ps, weights, c, bound)
+
+
+@pytest.mark.parametrize("weights", [[6e38, 6e38, -1.2e39], [1e-44, 1e-42, 0.0], [3e-45, 0.5, 0.25], [1e60, -1e60, 1.0]], ids=str)
+def test_f16_averages_with_weights_beyond_float32(weights):
+    from accdfl_amd.core.norms import wsum_bounded
+
+    large = max(abs(w) for w in weights) > 1
+    # powers of two: every product and sum of the definition is exact in 64 bits, so the large terms cancel to nothing
+    c = torch.zeros(1000, dtype=torch.float16, device="cuda")
+    ps = [torch.full_like(c, 0.125) for _ in weights]
+    out, _ = wsum_bounded(ps, weights, c, INF)
+    exact = torch.full((1000,), 0.125 * (1.0 if weights[0] == 1e60 else 0.0) if large else 0.125 * sum(weights), dtype=torch.float64)
+    no.assert_close(out, exact, 1000)
+    c = _rand(3001, "f16", 0.5, 1)
+    ps = [_rand(3001, "f16", 0.5, 2 + k) for k in range(len(weights))]
+    if large:
+        ps = [ps[0].clone() for _ in ps]
+    out, _ = wsum_bounded(ps, weights, c, INF)
+    if large:
+        # The terms cancel, but the rounding of products of 1e38 |d| and more to 64 bits, 2^-53 of them, is 1e22 |d|: any
+        # result of float16, infinities too, is within what 64 bits allow wherever |d| > 1e-15; d = 0 is exact.
+        d = ps[0].double() - c.double()
+        assert float(d[d != 0].abs().min()) > 1e-15
+        assert not bool(torch.isnan(out).any()) and torch.equal(out[d == 0], c[d == 0])
+    else:
+        _assert_average(out, ps, weights, c, INF)
+
+
+@pytest.mark.parametrize("n", [1, 2, 9, 128])
+@pytest.mark.parametrize("bound", [1.0, 1e-3, 1e-4, 1e-5, 1e-30])
+def test_an_outlier_of_any_size_is_bounded(bound, n):
+    """One peer of norm 3e38 and more moves the average by its weight times the bound, however small that is: its share,
+    near 1e-45 and below, is no normal float32."""
+    from accdfl_amd.core.norms import wsum_bounded
+
+    c = torch.zeros(2000, dtype=torch.bfloat16, device="cuda")
+    far = _rand(2000, "f64", 1e37, 3).to(torch.bfloat16)
+    far[777] = 3e38
+    peers = [far] + [c.clone() for _ in range(n - 1)]
+    out, _ = wsum_bounded(peers, [1.0 / 128] * n, c, bound)
+    # one term, no sum: within half a step of the definition
+    want = far.double().cpu() * (bound / no.norm([far]) / 128)
+    no.assert_close(out, want, 2000 + n)
+    assert abs(no.norm([out]) * 128 - bound) <= 2.0 ** -8 * bound
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [2, 5, 8, 11, 70])
+def test_an_outlier_beside_ordinary_peers(n, dtype):
+    """The round that holds a peer beyond float32 and the others alike are off by no more than any other round."""
+    from accdfl_amd.core.norms import wsum_bounded, wsum_bounded_multi
+
+    sizes = [5, 1025, 6007]
+    center, models, weights = _round(n, sizes, dtype, seed=21)
+    for t in models[n // 2]:
+        t.copy_(_rand(t.shape, "f64", 1.0, 22).to(DT[dtype]) * (3e37 if dtype == "bf16" else 6e3))
+    outs = [torch.empty_like(c) for c in center]
+    got = wsum_bounded_multi(models, weights, center, 0.5, outs)
+    want, wn, added = no.bounded(models, weights, center, 0.5)
+    # a norm is returned in float32 (beyond its largest value: infinite) and judged in 64 bits
+    no.assert_norm(got, [w if w <= torch.finfo(torch.float32).max else INF for w in wn], sum(sizes))
+    for o, w, a in zip(outs, want, added):
+        no.assert_close(o, w, sum(sizes) + n, a)
+    out, _ = wsum_bounded([m[2] for m in models], weights, center[2], 0.5, out=center[2].clone())
+    _assert_average(out, [m[2] for m in models], weights, center[2], 0.5)
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_a_slab_with_an_outlier(own):
+    from accdfl_amd.core.peer_slab import PeerSlab
+
+    total, n = 30_011, 6
+    center = _rand(total, "bf16", 0.5, 31)
+    peers = [(center.double() + _rand(total, "f64", 0.1, 40 + k)).to(torch.bfloat16) for k in range(n)]
+    peers[2] = torch.full_like(center, -3e38)
+    slab = PeerSlab([(total,)], torch.bfloat16, capacity=n)
+    for p in peers:
+        slab.stage_flat(p)
+    around = center if own else peers[0]
+    weights = [1.0 / n] * n
+    for bound in (2.0, 1e-6, INF):
+        out, _ = slab.reduce_bounded(bound, weights, center=center if own else None)
+        _assert_average(out[:total], peers, weights, around, bound)
