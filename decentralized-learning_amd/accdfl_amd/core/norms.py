@@ -24,10 +24,14 @@ too): calls on several streams or threads do not meet, and a call captured into 
 """
 from __future__ import annotations
 
+import bisect
 import contextlib
 import ctypes
+import itertools
+import math
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
+import numpy as np
 import torch
 from torch import nn
 
@@ -143,17 +147,95 @@ def _check(lists: List[List[torch.Tensor]], names: Sequence[str]) -> torch.devic
     return device
 
 
+# Overlaps of outputs that are not dense: the library checks the memory that it is given, which for them is a copy.
+_OVERLAP_WORK = 1_000_000  # candidates NumPy may try for two views whose spans meet; beyond it they count as overlapping
+
+
+class _Elements:
+    """Where the elements of a tensor lie: ``axes`` (stride, size) in elements of ``size`` bytes from ``begin`` on, all
+    before ``end``.  NumPy takes it for an array; the memory is not touched."""
+
+    def __init__(self, begin: int, axes: List[Tuple[int, int]], size: int):
+        self.begin, self.axes, self.size = begin, axes, size
+        self.end = begin + (sum(st * (n - 1) for st, n in axes) + 1) * size
+        self.step = math.gcd(*[st for st, _ in axes]) * size
+
+    @classmethod
+    def of(cls, t: torch.Tensor) -> "_Elements":
+        return cls(t.data_ptr(), [(st, n) for st, n in zip(t.stride(), t.shape) if n != 1], t.element_size())
+
+    def same(self, other: "_Elements") -> bool:
+        return self.begin == other.begin and self.axes == other.axes
+
+    @property
+    def __array_interface__(self):
+        return {"version": 3, "typestr": "|V%d" % self.size, "data": (self.begin, True),
+                "shape": tuple(n for _, n in self.axes), "strides": tuple(st * self.size for st, _ in self.axes)}
+
+    def meet(self, other: "_Elements") -> bool:
+        """Is there a byte that both have?"""
+        if self.end <= other.begin or other.end <= self.begin:
+            return False
+        step = math.gcd(self.step, other.step)
+        # both are periodic in `step` bytes: side by side in each period (columns of one matrix) they do not meet
+        if step and self.size <= (other.begin - self.begin) % step <= step - other.size:
+            return False
+        try:
+            return np.shares_memory(np.asarray(self), np.asarray(other), max_work=_OVERLAP_WORK)
+        except np.exceptions.TooHardError:
+            return True
+
+    def meets_itself(self) -> bool:
+        """Do two elements share memory?  Axis by axis, the smallest step first: what the axes so far reach, moved by any
+        number of steps of the next one that stays within that reach, may not meet itself."""
+        reach, inner = 0, []
+        for stride, n in sorted(self.axes):
+            if stride == 0:
+                return True
+            for k in range(1, min(n - 1, reach // stride) + 1):
+                if _Elements(self.begin, inner, self.size).meet(_Elements(self.begin + k * stride * self.size, inner, self.size)):
+                    return True
+            inner.append((stride, n))
+            reach += (n - 1) * stride
+        return False
+
+
+def _refuse_overlaps(lists: List[List[torch.Tensor]], names: Sequence[str], out: int) -> None:
+    """The library's rule for any strides: no element of lists[out] is written twice, and none is an element of another
+    tensor, but for the tensor in its own place of another list."""
+    places = [[_Elements.of(t) if t.numel() else None for t in ts] for ts in lists]
+    outs = sorted(((p, i) for i, p in enumerate(places[out]) if p), key=lambda o: o[0].begin)
+    for p, i in outs:
+        if p.meets_itself():
+            raise ValueError("%s tensor %d: an output has elements that share memory" % (names[out], i))
+    begins = [p.begin for p, _ in outs]
+    reach = list(itertools.accumulate((p.end for p, _ in outs), max))  # of outs[:j + 1]
+
+    def refuse(l, i, place, stop):
+        """Raises if tensor i of list l meets one of outs[:stop]."""
+        j = min(stop, bisect.bisect_left(begins, place.end)) - 1
+        while j >= 0 and reach[j] > place.begin:
+            if outs[j][0].meet(place):
+                raise _lib.DlaggError("%s tensor %d overlaps %s tensor %d" % (names[l], i, names[out], outs[j][1]))
+            j -= 1
+
+    for q, (p, i) in enumerate(outs):
+        refuse(out, i, p, q)
+    for l, ps in enumerate(places):
+        for i, p in enumerate(ps):
+            if l != out and p is not None and not p.same(places[out][i]):
+                refuse(l, i, p, len(outs))
+
+
 def _pack_checked(lists: List[List[torch.Tensor]], names: Sequence[str], lead: int, out: int = -1):
     """(tables, copies to write back) for any lists that _check accepts: tensors that are not dense, or whose
     element order differs within their place, are replaced by contiguous copies; lists[out]'s replacements are
-    returned as (tensor, its copy) to be copied back after the call."""
+    returned as (tensor, its copy) to be copied back after the call.  Outputs that overlap are refused."""
     device = _check(lists, names)
     lists = [list(ts) for ts in lists]
     back = []
     if out >= 0:
-        for t in lists[out]:
-            if any(st == 0 and sz > 1 for st, sz in zip(t.stride(), t.shape)):
-                raise ValueError("an output has elements that share memory (an expanded tensor)")
+        _refuse_overlaps(lists, names, out)
     for i in range(len(lists[0])):
         place = [ts[i] for ts in lists]
         if all(_dense(t) and not t.is_neg() and _same_order(t, place[0]) for t in place):

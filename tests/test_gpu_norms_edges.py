@@ -126,3 +126,81 @@ def test_a_slab_with_an_outlier(own):
     for bound in (2.0, 1e-6, INF):
         out, _ = slab.reduce_bounded(bound, weights, center=center if own else None)
         _assert_average(out[:total], peers, weights, around, bound)
+
+
+# ------------------------------------------------------------------------------------------ overlapping outputs
+def _overlapping():
+    """(name, the tensors to write): each list has an element that is written twice."""
+    buf = torch.arange(120, dtype=torch.float32, device="cuda")
+    m = buf.view(10, 12)
+    gapped = m[:, :3]
+    return [
+        ("the same view twice", [gapped, gapped]),
+        ("columns that cross", [m[:, :3], m[:, 2:5]]),
+        ("steps of two and four", [buf[::2], buf[::4]]),
+        ("a column of a whole", [m, m[:, 3:4]]),
+        ("dense beside gapped", [buf[:24], m[:, 11]]),
+        ("windows", [buf.as_strided((3, 3), (1, 1))]),
+        ("a window that meets itself late", [buf.as_strided((5, 4), (3, 4))]),
+        ("rows and their transpose", [m[:5, :5], m[:5, :5].t()]),
+    ]
+
+
+def test_overlapping_outputs_with_gaps_are_refused():
+    from accdfl_amd import _lib
+    from accdfl_amd.core.norms import clip_global_norm, clip_global_norm_, wsum_bounded_multi
+
+    for name, outs in _overlapping():
+        base = outs[0]._base if outs[0]._base is not None else outs[0]
+        before = base.clone()
+        versions = [o._version for o in outs]
+        fresh = [torch.ones(o.shape, device="cuda") for o in outs]
+        for call in (lambda: clip_global_norm_(outs, 0.1), lambda: clip_global_norm(fresh, 0.1, outs=outs),
+                     lambda: wsum_bounded_multi([fresh], [0.5], fresh, 1.0, outs),
+                     lambda: wsum_bounded_multi([outs], [0.5], outs, 1.0, outs)):
+            with pytest.raises((ValueError, _lib.DlaggError), match="overlap|share memory"):
+                call()
+            assert torch.equal(base, before), name
+        assert [o._version for o in outs] == versions, name
+
+
+def test_outputs_that_cross_other_inputs_are_refused():
+    from accdfl_amd import _lib
+    from accdfl_amd.core.norms import clip_global_norm, wsum_bounded_multi
+
+    m = _rand((10, 12), "f32", 1.0, 3)
+    fresh = torch.ones(10, 3, device="cuda")
+    for tensors, outs in (([m[:, :3]], [m[:, 1:4]]), ([m[:, :3], m[:, 3:6]], [m[:, 3:6], fresh]),
+                          ([m[:5, :5]], [m[:5, :5].t()]), ([m[:3, :3].expand(3, 3)], [m[:6:2, :3]])):
+        before = m.clone()
+        with pytest.raises(_lib.DlaggError, match="overlap"):
+            clip_global_norm(tensors, 0.1, outs=outs)
+        with pytest.raises(_lib.DlaggError, match="overlap"):
+            wsum_bounded_multi([tensors], [1.0], tensors, 0.1, outs)
+        assert torch.equal(m, before)
+
+
+def test_interleaved_views_of_one_base_are_not_refused():
+    """Views with gaps that share no element: columns, rows, every other element, and one that lies in another's gaps."""
+    from accdfl_amd.core.norms import clip_global_norm_, wsum_bounded_multi
+
+    def views(m):
+        crossed = m.as_strided((2, 2), (3, 2), m.storage_offset() + 9 * 12 + 6)  # columns 6, 8, 9 and 11 of row 9
+        return [m[:, 0], m[:, 1:4], m[::2, 4:6], m[1::2, 4:6], m.view(-1)[7::12], m[3:4, 8:10], crossed]
+
+    m = _rand((12, 12), "f32", 1.0, 5)
+    rest = torch.ones_like(m, dtype=torch.bool)
+    for v in views(rest):
+        v.zero_()
+    kept = m.clone()
+    want, _ = no.clip(views(m), 0.2)
+    clip_global_norm_(views(m), 0.2)
+    for v, w in zip(views(m), want):
+        no.assert_close(v, w, 144)
+    assert torch.equal(m[rest], kept[rest])
+    peer = _rand((12, 12), "f32", 1.0, 6)
+    want, wn, added = no.bounded([views(peer)], [0.5], views(m), 0.3)
+    wsum_bounded_multi([views(peer)], [0.5], views(m), 0.3, views(m))
+    for v, w, a in zip(views(m), want, added):
+        no.assert_close(v, w, 144, a)
+    assert torch.equal(m[rest], kept[rest])

@@ -1,0 +1,63 @@
+"""The norm operators' rules at their edges, for what needs no GPU: which views overlap, how large a launch is, and the
+staging of rounds of CPU models."""
+import itertools
+import random
+
+import pytest
+import torch
+
+
+def _bytes_of(t):
+    size = t.element_size()
+    return [t.data_ptr() + size * sum(i * st for i, st in zip(at, t.stride())) + b
+            for at in itertools.product(*[range(n) for n in t.shape]) for b in range(size)]
+
+
+def test_overlaps_are_told_from_neighbours():
+    """Random views of one buffer, of three element sizes, against their bytes."""
+    from accdfl_amd.core.norms import _Elements
+
+    buf = torch.zeros(400)
+    bases = [buf, buf.view(torch.int16), buf.view(torch.int64)]
+    rng = random.Random(1)
+
+    def view():
+        axes, times = rng.randint(0, 3), rng.choice([1, 1, 2, 3, 4])
+        return rng.choice(bases).as_strided([rng.randint(1, 4) for _ in range(axes)],
+                                            [times * rng.randint(0, 5) for _ in range(axes)], rng.randint(0, 60))
+    met = itself = 0
+    for _ in range(4000):
+        a, b = view(), view()
+        ba, bb = _bytes_of(a), _bytes_of(b)
+        assert _Elements.of(a).meets_itself() == (len(set(ba)) < len(ba)), (a.shape, a.stride())
+        assert _Elements.of(a).meet(_Elements.of(b)) == bool(set(ba) & set(bb)), (a.shape, a.stride(), b.shape, b.stride())
+        met += bool(set(ba) & set(bb))
+        itself += len(set(ba)) < len(ba)
+    assert met > 300 and itself > 300
+
+
+def test_refusals_of_views_by_their_elements():
+    from accdfl_amd import _lib
+    from accdfl_amd.core.norms import _refuse_overlaps
+
+    m = torch.zeros(10, 12)
+    fresh = torch.zeros(10, 3)
+    fine = [
+        ([m[:, :3], m[:, 3:6]], [m[:, :3], m[:, 3:6]]),            # in place
+        ([fresh, fresh], [m[:, :3], m[:, 3:6]]),                   # an input twice
+        ([m[:, 6:9], m[:, 6:9]], [m[:, :3], m[:, 3:6]]),           # in the gaps of the outputs
+        ([torch.zeros(0)], [m[:0, 0]]),
+    ]
+    for ins, outs in fine:
+        _refuse_overlaps([ins, outs], ["tensors", "outs"], 1)
+    for ins, outs, what in (
+            ([fresh, fresh], [m[:, :3], m[:, 2:5]], "outs tensor [01] overlaps outs tensor [01]"),
+            ([fresh, fresh], [m[:, :3], m[:, :3]], "outs tensor [01] overlaps outs tensor [01]"),
+            ([m[:, 3:6], m[:, :3]], [m[:, :3], m[:, 3:6]], "tensors tensor 0 overlaps outs tensor 1"),
+            ([m[:, 1:4]], [m[:, :3]], "tensors tensor 0 overlaps outs tensor 0"),
+            ([m[:5, :5]], [m[:5, :5].t()], "tensors tensor 0 overlaps outs tensor 0")):
+        with pytest.raises(_lib.DlaggError, match=what):
+            _refuse_overlaps([ins, outs], ["tensors", "outs"], 1)
+    for out in (m[:, :1].expand(10, 3), m.as_strided((3, 3), (1, 1)), m.as_strided((5, 4), (3, 4))):
+        with pytest.raises(ValueError, match="outs tensor 0: an output has elements that share memory"):
+            _refuse_overlaps([[torch.zeros(out.shape)], [out]], ["tensors", "outs"], 1)
