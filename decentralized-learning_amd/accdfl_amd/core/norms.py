@@ -50,11 +50,12 @@ class _Tables:
     for when the extension is absent: ``n`` tensors on HIP device ``device``; dtype codes, counts, the addresses of
     the first lists, and those of the other lists tensor-major."""
 
-    def __init__(self, device: int, lists: List[List[torch.Tensor]], lead: int):
+    def __init__(self, device: int, lists: List[List[torch.Tensor]], lead: int, written: Sequence[torch.Tensor]):
         n, rest = len(lists[0]), lists[lead:]
         address = lambda t: t.data_ptr() if t.numel() else 0  # noqa: E731
         self.n = n
         self.device = device
+        self.written = [t for t in written if not t.is_inference()]
         self.wide = any(t.dtype == torch.float64 for t in lists[0])
         self.codes = (ctypes.c_int * n)(*[_wsum.dtype_code(t.dtype) for t in lists[0]])
         self.numels = (ctypes.c_int64 * n)(*[t.numel() for t in lists[0]])
@@ -64,8 +65,11 @@ class _Tables:
     def _result(self, size, double: bool):
         return torch.empty(size, dtype=torch.float64 if double else torch.float32, device=self.device)
 
-    def _call(self, name: str, out, *args):
-        return getattr(_lib.lib().so, name)(self.n, self.codes, *args), out
+    def _call(self, name: str, out, *args, written: Sequence[torch.Tensor] = ()):
+        rc = getattr(_lib.lib().so, name)(self.n, self.codes, *args)
+        if rc >= 0:  # not refused
+            torch.autograd.graph.increment_version(written)
+        return rc, out
 
     def norm(self, fn, code, counter, nbytes, stream):
         out, ws = self._result((), self.wide), _workspace(nbytes, self.device)
@@ -75,7 +79,7 @@ class _Tables:
     def clip(self, fn, code, max_norm, eps, counter, nbytes, stream):
         out, ws = self._result((), self.wide), _workspace(nbytes, self.device)
         return self._call("dla_norm_clip", out, self.lead[0], self.lead[1], self.numels, code, max_norm, eps,
-                          3 * self.wide, out.data_ptr(), counter, ws.data_ptr(), nbytes, stream)
+                          3 * self.wide, out.data_ptr(), counter, ws.data_ptr(), nbytes, stream, written=self.written)
 
     def peer_norms(self, fn, n, squared, counters, table, table_bytes, nbytes, stream):
         out, ws = self._result(n, squared or self.wide), _workspace(nbytes, self.device)
@@ -87,14 +91,14 @@ class _Tables:
         out, ws = self._result(len(weights), self.wide), _workspace(nbytes, self.device)
         return self._call("dla_wsum_bounded", out, self.rest, self.lead[0], self.lead[1], self.numels,
                           _lib._dbl_array(weights), len(weights), max_norm, sq, 3 * self.wide, out.data_ptr(), counters,
-                          table, table_bytes, ws.data_ptr(), nbytes, stream)
+                          table, table_bytes, ws.data_ptr(), nbytes, stream, written=self.written)
 
 
-def _pack(lists: List[List[torch.Tensor]], lead: int, bump: int = -1):
-    """The tables of lists whose tensors the kernels take as they are (walk.cpp dense_lists), else None.
-    ``bump``: the list that the call writes (its tensors' version counters move on)."""
+def _pack(lists: List[List[torch.Tensor]], lead: int, out: int = -1):
+    """The tables of lists whose tensors the kernels take as they are (walk.cpp dense_lists), else None.  ``out``: the
+    list that the call writes (its tensors' version counters then move on, unless the call is refused)."""
     mod = _lib.walk_module()
-    return None if mod is None else mod.dense_lists(lists, lead, bump)
+    return None if mod is None else mod.dense_lists(lists, lead, out)
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -248,9 +252,7 @@ def _pack_checked(lists: List[List[torch.Tensor]], names: Sequence[str], lead: i
                 back.append((place[out], lists[out][i]))
     tables = _pack(lists, lead, out)
     if tables is None:
-        tables = _Tables(device.index, lists, lead)
-        if out >= 0:
-            torch.autograd.graph.increment_version([t for t in lists[out] if not t.is_inference()])
+        tables = _Tables(device.index, lists, lead, lists[out] if out >= 0 else ())
     return tables, back, lists  # the lists keep the copies alive until the call is enqueued
 
 
@@ -392,7 +394,7 @@ def clip_global_norm(tensors: Tensors, max_norm: float, norm_type: float = 2.0, 
             raise ValueError("clip_global_norm: %d outs for %d tensors" % (len(outs), len(tensors)))
         if not tensors:
             return list(outs), torch.zeros((), dtype=torch.float32, device=_device_of(tensors, stream))
-        tables, back, keep = _pack([tensors, outs], 2, bump=1), (), None
+        tables, back, keep = _pack([tensors, outs], 2, out=1), (), None
         if tables is None:
             tables, back, keep = _pack_checked([tensors, outs], ["tensors", "outs"], 2, out=1)
         raw = _raw_stream(tables.device)
@@ -429,7 +431,7 @@ def clip_grad_norm_(parameters: Tensors, max_norm: float, norm_type: float = 2.0
 
 # ----------------------------------------------------------------------------------------- peers around a centre
 def _pack_round(lists: List[List[torch.Tensor]], names, lead: int, out: int = -1):
-    tables = _pack(lists, lead, bump=out)
+    tables = _pack(lists, lead, out)
     if tables is not None:
         return tables, (), None
     return _pack_checked(lists, names() if callable(names) else names, lead, out=out)

@@ -248,6 +248,7 @@ struct DenseTables {
   std::vector<int64_t> numels;
   std::vector<uint64_t> head;  // addresses [lead][n] of the first `lead` lists
   std::vector<uint64_t> tail;  // addresses [n][L - lead] of the others
+  std::vector<at::Tensor> written;  // what a call writes
   const uint64_t* lead(py::ssize_t i) const { return head.data() + i * n; }
 
   at::Tensor result(at::IntArrayRef sizes, bool doubles) const {
@@ -264,6 +265,13 @@ struct DenseTables {
     return reinterpret_cast<Fn>(fn)(args...);
   }
   int out_code() const { return wide ? 3 : 0; }  // DLA_F64 : DLA_F32
+  // After a call that was not refused (a refusal is negative and has launched nothing): the version counters of what it
+  // writes move on, as torch's own in-place operators do it.
+  void moved_on(int rc) const {
+    if (rc < 0) return;
+    for (const at::Tensor& x : written)
+      if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+  }
 
   // dla_norm: (status, the norm)
   py::tuple norm(uint64_t fn, int norm_code, uint64_t counter, int64_t ws_bytes, uint64_t stream) const {
@@ -284,6 +292,7 @@ struct DenseTables {
         fn, static_cast<int>(n), codes.data(), reinterpret_cast<const void* const*>(lead(0)),
         reinterpret_cast<void* const*>(const_cast<uint64_t*>(lead(1))), numels.data(), norm_code, max_norm, eps,
         out_code(), out.data_ptr(), ptr(counter), ws.data_ptr(), ws_bytes, ptr(stream));
+    moved_on(rc);
     return py::make_tuple(rc, out);
   }
   // dla_peer_norms of the other lists around the first: (status, norms or float64 squares)
@@ -323,6 +332,7 @@ struct DenseTables {
         reinterpret_cast<const void* const*>(lead(0)), reinterpret_cast<void* const*>(const_cast<uint64_t*>(to)),
         numels.data(), weights.data(), n_peers, max_norm, reinterpret_cast<const double*>(sq), out_code(), out.data_ptr(),
         ptr(counters), ptr(table), table_bytes, ws.data_ptr(), ws_bytes, ptr(stream));
+    moved_on(rc);
     return py::make_tuple(rc, out);
   }
 };
@@ -381,9 +391,8 @@ std::unique_ptr<DenseTables> pack_lists(const std::vector<std::vector<PyObject*>
 }
 
 // pack_lists of Python lists, or None (the caller's own pass then says which tensor does not fit, or copies it).
-// The tensors of lists[bump] (-1: none) are about to be written: their version counters move on, as torch's own
-// in-place operators do it.
-py::object dense_lists(py::list lists, py::ssize_t lead, py::ssize_t bump) {
+// lists[writes] (-1: none) is what the call writes.
+py::object dense_lists(py::list lists, py::ssize_t lead, py::ssize_t writes) {
   const py::ssize_t n_lists = PyList_GET_SIZE(lists.ptr());
   if (n_lists < 1 || lead < 1 || lead > n_lists) return py::none();
   std::vector<std::vector<PyObject*>> all(n_lists);
@@ -397,11 +406,9 @@ py::object dense_lists(py::list lists, py::ssize_t lead, py::ssize_t bump) {
   if (all[0].empty()) return py::none();
   auto tables = pack_lists(all, static_cast<size_t>(lead));
   if (!tables) return py::none();
-  if (bump >= 0 && bump < n_lists) {
-    for (PyObject* o : all[bump]) {
-      const at::Tensor& x = THPVariable_Unpack(o);
-      if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
-    }
+  if (writes >= 0 && writes < n_lists) {
+    tables->written.reserve(all[writes].size());
+    for (PyObject* o : all[writes]) tables->written.push_back(THPVariable_Unpack(o));
   }
   return py::cast(std::move(tables));
 }
@@ -1760,7 +1767,7 @@ PYBIND11_MODULE(_dla_walk, m) {
       .def("clip", &DenseTables::clip)
       .def("peer_norms", &DenseTables::peer_norms)
       .def("bounded", &DenseTables::bounded);
-  m.def("dense_lists", &dense_lists, py::arg("lists"), py::arg("lead"), py::arg("bump"));
+  m.def("dense_lists", &dense_lists, py::arg("lists"), py::arg("lead"), py::arg("writes"));
   m.def("module_tables", &module_tables, py::arg("models"), py::arg("plain"));
   m.def("block_table", &block_table, py::arg("blocks"));
   m.def("fingerprint", &fingerprint, py::arg("model"), py::arg("plain"));

@@ -204,3 +204,55 @@ def test_interleaved_views_of_one_base_are_not_refused():
     for v, w, a in zip(views(m), want, added):
         no.assert_close(v, w, 144, a)
     assert torch.equal(m[rest], kept[rest])
+
+
+# ------------------------------------------------------------------------------- what a refused clip leaves alone
+def _bits(t):
+    return t.view({2: torch.int16, 4: torch.int32, 8: torch.int64}[t.element_size()]).clone()
+
+
+@pytest.mark.parametrize("p", [2.0, 1.0, INF])
+@pytest.mark.parametrize("bad", [math.nan, INF, -INF])
+def test_a_clip_refused_for_its_norm_writes_nothing(bad, p):
+    from accdfl_amd.core.norms import clip_global_norm, clip_global_norm_
+
+    for dtype in DT:
+        base = _rand((50, 40), dtype, 1.0, 2)
+        ts = [_rand(9, dtype), _rand(70_001, dtype, 1.0, 1), base[:, 3:20]]  # the last is written through a copy
+        ts[1][33_333] = bad
+        sent = [torch.full_like(t, 7.0) for t in ts]
+        before, versions = [_bits(t) for t in ts + sent], [t._version for t in ts + sent]
+        with pytest.raises(RuntimeError, match="not finite"):
+            clip_global_norm_(ts, 1.0, p, error_if_nonfinite=True)
+        with pytest.raises(RuntimeError, match="not finite"):
+            clip_global_norm(ts, 1.0, p, error_if_nonfinite=True, outs=sent)
+        assert all(torch.equal(_bits(t), b) for t, b in zip(ts + sent, before))
+        assert [t._version for t in ts + sent] == versions
+        ts[1][33_333] = 0.0
+        versions = [t._version for t in ts]
+        want, wn = no.clip(ts, 1.0, p)
+        no.assert_norm(clip_global_norm_(ts, 1.0, p, error_if_nonfinite=True), wn, 80_000)
+        for t, w in zip(ts, want):
+            no.assert_close(t, w, 80_000)
+        assert all(t._version > v for t, v in zip(ts, versions))
+
+
+def test_a_refused_call_moves_no_version():
+    from accdfl_amd import _lib
+    from accdfl_amd.core.norms import clip_global_norm_, wsum_bounded
+
+    t = _rand(100)
+    views = [t[:60], t[50:]]
+    with pytest.raises(_lib.DlaggError, match="overlap"):
+        clip_global_norm_(views, 0.1)
+    with pytest.raises(_lib.DlaggError, match="overlap"):
+        wsum_bounded([t[:50]], [1.0], t[:50], 1.0, out=t[1:51])
+    assert t._version == 0
+
+
+def test_without_the_walk_extension_a_refused_call_moves_no_version(monkeypatch):
+    from accdfl_amd import _lib
+
+    monkeypatch.setattr(_lib, "walk_module", lambda: None)
+    test_a_refused_call_moves_no_version()
+    test_a_clip_refused_for_its_norm_writes_nothing(math.nan, 2.0)
