@@ -390,6 +390,8 @@ class PeerSlab:
                                              None if row is None else row.data_ptr(), weights, self.total, bound,
                                              out.data_ptr(), _lib.DLA_F64 if wide else _lib.DLA_F32, norms.data_ptr(),
                                              _norms._counter(self.device.index, raw), ws.data_ptr(), nbytes, raw)
+            if not out.is_inference():  # written by address: torch sees it by its version counter, as on a slab of rows
+                torch.autograd.graph.increment_version(out)
         return out, norms
 
     def reduce_bounded_into(self, params: Sequence[torch.Tensor], max_norm: float,

@@ -256,3 +256,21 @@ def test_without_the_walk_extension_a_refused_call_moves_no_version(monkeypatch)
     monkeypatch.setattr(_lib, "walk_module", lambda: None)
     test_a_refused_call_moves_no_version()
     test_a_clip_refused_for_its_norm_writes_nothing(math.nan, 2.0)
+
+
+# ---------------------------------------------------------------------------------------- what is written has moved on
+@pytest.mark.parametrize("dtype", list(DT))
+def test_a_slab_s_output_has_moved_on(dtype):
+    from accdfl_amd.core.peer_slab import PeerSlab
+
+    slab = PeerSlab([(5003,)], DT[dtype], capacity=3)
+    for k in range(3):
+        slab.stage_flat(_rand(5003, dtype, 1.0, k))
+    out = torch.zeros(5003, dtype=DT[dtype], device="cuda")
+    version = out._version
+    assert slab.reduce_bounded(0.5, out=out)[0] is out and out._version > version
+    w = torch.ones(5003, dtype=DT[dtype], device="cuda", requires_grad=True)
+    loss = (w * out).sum()
+    slab.reduce_bounded(0.25, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
