@@ -338,19 +338,26 @@ class PeerSlab:
     def _center_row(self, center) -> torch.Tensor:
         """A centre — the slab's flat layout on the device, or tensors of the slab's layout anywhere — as a flat
         device vector of ``total`` elements."""
-        if isinstance(center, torch.Tensor):
-            if (center.dtype != self.dtype or center.numel() != self.total or center.device != self.device
-                    or not center.is_contiguous()):
-                raise ValueError("center must be a contiguous %s tensor of %d elements on %s"
-                                 % (self.dtype, self.total, self.device))
-            return center.detach().view(-1)
-        center = list(center)
-        if not self.matches(center):
+        from accdfl_amd.core import norms as _norms
+
+        flat = isinstance(center, torch.Tensor)
+        parts = [center] if flat else list(center)
+        if flat and (center.dtype != self.dtype or center.numel() != self.total or center.device != self.device
+                     or not center.is_contiguous()):
+            raise ValueError("center must be a contiguous %s tensor of %d elements on %s"
+                             % (self.dtype, self.total, self.device))
+        if not flat and not self.matches(parts):
             raise ValueError("PeerSlab: the centre's parameter layout differs from the slab's")
-        if not center:
+        for p in parts:
+            if not _norms._held(p):
+                raise ValueError("PeerSlab: a tensor of the centre lies outside its storage (%d bytes)"
+                                 % p.untyped_storage().nbytes())
+        if flat:
+            return center.detach().resolve_neg().view(-1)
+        if not parts:
             return torch.empty(0, dtype=self.dtype, device=self.device)
-        row = torch.cat([p.detach().reshape(-1) for p in center]) if len({p.device for p in center}) == 1 else (
-            torch.cat([p.detach().reshape(-1).to(self.device) for p in center]))
+        row = torch.cat([p.detach().reshape(-1) for p in parts]) if len({p.device for p in parts}) == 1 else (
+            torch.cat([p.detach().reshape(-1).to(self.device) for p in parts]))
         return row.to(self.device)
 
     def reduce_bounded(self, max_norm: float, weights: Optional[Sequence[float]] = None, center=None,
@@ -375,12 +382,16 @@ class PeerSlab:
             if out.device != self.device or out.dtype != self.dtype or out.numel() < self.total or not out.is_contiguous():
                 raise ValueError("out must be a contiguous %s tensor of >= %d elements on %s"
                                  % (self.dtype, self.total, self.device))
+            if not _norms._held(out):
+                raise ValueError("out lies outside its storage (%d bytes)" % out.untyped_storage().nbytes())
             row = None if center is None else self._center_row(center)
             if self.layout == "rows":
                 rows = [self.buf[k, : self.total] for k in range(n)]
                 _, norms = _norms.wsum_bounded(rows, weights, rows[0] if row is None else row, bound,
                                                out=out.view(-1)[: self.total])
                 return out, norms
+            if out.is_neg():  # its memory is written by address
+                raise ValueError("out is a negated view")
             wide = self.dtype == torch.float64
             norms = torch.empty(n, dtype=torch.float64 if wide else torch.float32, device=self.device)
             nbytes = _lib.peer_workspace(1, n)

@@ -274,3 +274,29 @@ def test_a_slab_s_output_has_moved_on(dtype):
     slab.reduce_bounded(0.25, out=out)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("layout", ["tiled", "rows"])
+def test_a_slab_s_tensors_are_what_their_storages_hold(layout):
+    from accdfl_amd.core.peer_slab import PeerSlab
+
+    slab = PeerSlab([(40, 50), (3,)], torch.float32, capacity=2, layout=layout)
+    peers = [_rand(2003, "f32", 1.0, k) for k in range(2)]
+    for p in peers:
+        slab.stage_flat(p)
+    freed = torch.ones(2003, device="cuda")
+    part, whole = freed[:2000].view(40, 50), torch.ones(3, device="cuda")
+    freed.untyped_storage().resize_(0)
+    for kw in (dict(out=freed), dict(center=freed), dict(center=[part, whole])):
+        with pytest.raises(ValueError, match="storage"):
+            slab.reduce_bounded(1.0, **kw)
+    # a negated view is read, and where it can be written, as what it stands for
+    center, out = _rand(2003, "f32", 1.0, 9), torch.zeros(2003, device="cuda")
+    if layout == "tiled":
+        with pytest.raises(ValueError, match="negated"):
+            slab.reduce_bounded(1.0, out=torch._neg_view(out))
+    else:
+        slab.reduce_bounded(1.0, [0.5, 0.5], center=center, out=torch._neg_view(out))
+        _assert_average(-out, peers, [0.5, 0.5], center, 1.0)
+    out, _ = slab.reduce_bounded(1.0, [0.5, 0.5], center=torch._neg_view(center))
+    _assert_average(out, peers, [0.5, 0.5], -center, 1.0)
