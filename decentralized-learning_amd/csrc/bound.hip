@@ -795,7 +795,7 @@ int64_t list_units(int dt, int64_t n, int vec) {
   return (n + per - 1) / per;
 }
 
-// `most` workgroups in all, shared by the launches as their units are, or (0) one per unit.
+// `most` workgroups in all, shared by the launches as their units are, or (0) one per unit where a launch takes that many.
 bool plan_list(const std::vector<int>& order, const int* dtypes, const int64_t* numels, int vec, int per_launch, int64_t most,
                std::vector<ListLaunch>* out) {
   int64_t total = 0;
@@ -805,7 +805,7 @@ bool plan_list(const std::vector<int>& order, const int* dtypes, const int64_t* 
     int64_t units = 0;
     for (int q = static_cast<int>(i); q < end; ++q) units += list_units(dtypes[order[q]], numels[order[q]], vec);
     if (units > 0xffffffffll) return false;
-    const int64_t share = most ? std::max<int64_t>(1, most * units / total) : 0x7fffffff;
+    const int64_t share = most ? std::max<int64_t>(1, most * units / total) : dla_internal_grid(units, kThreads);
     out->push_back({static_cast<int>(i), end, static_cast<uint32_t>(units), static_cast<int>(std::min(units, share))});
   }
   return true;
@@ -1200,7 +1200,7 @@ int round_impl(const char* what, const Round& r, double max_norm, const double* 
     if (hipError_t e = hipGetLastError()) return hip_fail(what, e);
   }
   if (!r.outs || m == 0) return DLA_OK;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(mean_units, 0x7fffffff)));
+  const dim3 grid(static_cast<unsigned>(dla_internal_grid(mean_units, kMeanThreads)));
   // One wave per workgroup and 8 + 1 loads in flight per wave: beyond some 100 KB in flight per CU more waves only
   // keep more DRAM rows open at once.  Rounds of 8 peers and more that read over the Infinity Cache's 256 MB run
   // 14 waves per CU, by reserving LDS that nothing reads (us, 14 / uncapped: 8 x 25 M f32 157 / 165, 16 x ResNet-34

@@ -300,3 +300,27 @@ def test_a_slab_s_tensors_are_what_their_storages_hold(layout):
         _assert_average(-out, peers, [0.5, 0.5], center, 1.0)
     out, _ = slab.reduce_bounded(1.0, [0.5, 0.5], center=torch._neg_view(center))
     _assert_average(out, peers, [0.5, 0.5], -center, 1.0)
+
+
+# ------------------------------------------------------------------------------------------------------- 64 GiB
+def test_an_average_of_64_gib_and_more():
+    """One more unit than a launch has workgroups for: the first ones walk.  In place, around the output."""
+    from accdfl_amd.core.norms import wsum_bounded
+
+    n = 2 ** 26 * 512 + 517
+    if torch.cuda.mem_get_info()[0] < 2 * 2 * n + (8 << 30):
+        pytest.skip("needs 136 GiB of free memory")
+    center = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    peer = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    at = [0, 1, 511, 512, 513, 1023, 1024, 1500, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, n // 2, n - 518, n - 6, n - 5, n - 1]
+    for i, a in enumerate(at):
+        peer[a] = float(i + 1)
+        center[a] = 1.0
+    out, norms = wsum_bounded([peer], [0.5], center, INF, out=center)
+    got = [float(out[a]) for a in at]
+    rest = [float(out[a + 2].abs()) for a in at if a + 2 < n and a + 2 not in at]
+    no.assert_norm(norms, [math.sqrt(sum(i * i for i in range(len(at))))], 1000)
+    del center, peer, out
+    torch.cuda.empty_cache()
+    assert got == [1.0 + 0.5 * i for i in range(len(at))]
+    assert not any(rest)

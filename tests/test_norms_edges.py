@@ -1,7 +1,9 @@
 """The norm operators' rules at their edges, for what needs no GPU: which views overlap, how large a launch is, and the
 staging of rounds of CPU models."""
 import itertools
+import os
 import random
+import subprocess
 
 import pytest
 import torch
@@ -61,3 +63,27 @@ def test_refusals_of_views_by_their_elements():
     for out in (m[:, :1].expand(10, 3), m.as_strided((3, 3), (1, 1)), m.as_strided((5, 4), (3, 4))):
         with pytest.raises(ValueError, match="outs tensor 0: an output has elements that share memory"):
             _refuse_overlaps([[torch.zeros(out.shape)], [out]], ["tensors", "outs"], 1)
+
+
+def test_no_launch_has_more_threads_than_hip_takes(tmp_path):
+    """The grid of the kernels that give each unit a workgroup: an average of 64 GiB (2^26 units of 64 threads), a clip of
+    256 GiB (2^24 units of 256) and everything around them."""
+    from accdfl_amd import _lib
+
+    src = tmp_path / "grid.cpp"
+    src.write_text("""
+#include "dlagg_internal.h"
+#include <cstdio>
+#include <cstdlib>
+int main(int n, char** v) {
+  for (int i = 1; i + 1 < n; i += 2) std::printf("%lld\\n", (long long)dla_internal_grid(std::atoll(v[i]), std::atoi(v[i + 1])));
+}
+""")
+    exe = str(tmp_path / "grid")
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.dirname(_lib.CSRC_INTERNAL), "-o", exe, str(src)], check=True)
+    asked = [(units, threads) for threads in (64, 256) for power in (0, 10, 23, 24, 25, 26, 27, 31, 32, 53)
+             for units in (2 ** power - 1, 2 ** power, 2 ** power + 1)]
+    out = subprocess.run([exe] + [str(v) for pair in asked for v in pair], check=True, capture_output=True, text=True)
+    for (units, threads), grid in zip(asked, map(int, out.stdout.split())):
+        assert grid * threads < 2 ** 32 and grid <= units, (units, threads, grid)
+        assert grid == units or (grid + 1) * threads >= 2 ** 32, (units, threads, grid)
