@@ -18,6 +18,7 @@ and the centre must have the same parameters (count, shapes, dtypes).
 """
 from __future__ import annotations
 
+import contextlib
 import threading
 from typing import Dict, List, Optional
 
@@ -85,14 +86,30 @@ class _HostStage:
             self.events[i].record(stream)
 
 
-_host_stages: Dict[torch.device, _HostStage] = {}
-_host_lock = threading.Lock()
+# The stages that no round is using: rounds at once (threads, GPUs, a round made by a model's own __deepcopy__) each
+# have one of their own, and none waits for another's.
+_free_stages: Dict[torch.device, List[_HostStage]] = {}
+_stages_lock = threading.Lock()
+
+
+@contextlib.contextmanager
+def _host_stage(device: torch.device):
+    with _stages_lock:
+        free = _free_stages.get(device)
+        stage = free.pop() if free else None
+    if stage is None:
+        stage = _HostStage(device)
+    yield stage
+    # a round that failed does not come here: its stage goes, with copies that may not have ended
+    with _stages_lock:
+        _free_stages.setdefault(device, []).append(stage)
 
 
 def release_staging() -> None:
-    """Free the page-locked buffers of CPU rounds."""
-    with _host_lock:
-        _host_stages.clear()
+    """Free the page-locked buffers of CPU rounds (64 MiB for each of the most rounds that ran at once), but for those
+    that a round is using."""
+    with _stages_lock:
+        _free_stages.clear()
 
 
 class _Pieces:
@@ -135,10 +152,7 @@ def _host_round(models: List[nn.Module], weights, center: nn.Module, max_norm: f
     ingress = _Pieces(np.frombuffer(ptrs, dtype=np.int64), numels, esize, pitch)
     cur = torch.cuda.current_stream(device)
     buf = torch.empty(rows * pitch, dtype=torch.uint8, device=device)
-    with _host_lock:
-        stage = _host_stages.get(device)
-        if stage is None:
-            stage = _host_stages[device] = _HostStage(device)
+    with _host_stage(device) as stage:
         stream = cur if ingress.end <= stage.BYTES else stage.stream  # one piece: nothing to overlap
         stream.wait_stream(cur)
         try:

@@ -1,10 +1,12 @@
 """The norm operators at the ends of their ranges and of their contract: what a 16-bit average does with values and shares
 that float32 does not hold, which calls are refused, and what a refused call leaves as it was.  norms_oracle.py states the
 definitions and how far a correct result may be off.  Run on the MI355X: -m gpu."""
+import copy
 import math
 
 import pytest
 import torch
+from torch import nn
 
 import norms_oracle as no
 from test_gpu_norms import DT, INF, _list, _native, _rand, _round  # noqa: F401 (the fixture is used by being here)
@@ -324,3 +326,38 @@ def test_an_average_of_64_gib_and_more():
     torch.cuda.empty_cache()
     assert got == [1.0 + 0.5 * i for i in range(len(at))]
     assert not any(rest)
+
+
+# ------------------------------------------------------------------------------------------------ CPU rounds at once
+class _Nested(nn.Module):
+    """Averages other models while it is being copied."""
+
+    def __init__(self, seed, others=()):
+        super().__init__()
+        self.w = nn.Parameter(_rand((300, 40), "f32", 0.1, seed).cpu())
+        self.others, self.made = others, []
+
+    def __deepcopy__(self, memo):
+        twin = _Nested.__new__(_Nested)
+        memo[id(self)] = twin
+        nn.Module.__init__(twin)
+        twin.others, twin.made = (), []
+        twin.w = copy.deepcopy(self.w, memo)
+        if self.others:
+            from accdfl_amd.core.gradient_aggregation.norm_bounded import NormBoundedFedAvg
+
+            self.made.append(NormBoundedFedAvg(1.0).aggregate(list(self.others), None))
+        return twin
+
+
+def test_a_cpu_round_within_a_cpu_round():
+    from accdfl_amd.core.gradient_aggregation.norm_bounded import NormBoundedFedAvg, release_staging
+
+    others = [_Nested(50 + k) for k in range(3)]
+    models = [_Nested(60, others)] + [_Nested(61 + k) for k in range(2)]
+    out = NormBoundedFedAvg(2.0).aggregate(models, [0.5, 0.25, 0.25])
+    (inner,) = models[0].made
+    for got, ms, weights, bound in ((out, models, [0.5, 0.25, 0.25], 2.0), (inner, others, [1 / 3] * 3, 1.0)):
+        want, _, added = no.bounded([[m.w] for m in ms], weights, [ms[0].w], bound)
+        no.assert_close(got.w, want[0], 12_000, added[0])
+    release_staging()

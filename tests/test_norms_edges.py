@@ -87,3 +87,23 @@ int main(int n, char** v) {
     for (units, threads), grid in zip(asked, map(int, out.stdout.split())):
         assert grid * threads < 2 ** 32 and grid <= units, (units, threads, grid)
         assert grid == units or (grid + 1) * threads >= 2 ** 32, (units, threads, grid)
+
+
+def test_stages_of_rounds_at_once(monkeypatch):
+    """A round that begins within another one, in any thread, has a stage of its own; they are kept for later rounds, but
+    not that of a round that failed."""
+    from accdfl_amd.core.gradient_aggregation import norm_bounded as nb
+
+    monkeypatch.setattr(nb, "_HostStage", lambda device: object())
+    monkeypatch.setattr(nb, "_free_stages", {})
+    with nb._host_stage(0) as a:
+        with nb._host_stage(0) as b, nb._host_stage(1) as c:
+            assert len({id(a), id(b), id(c)}) == 3
+    with nb._host_stage(0) as first, nb._host_stage(0) as second:
+        assert {id(first), id(second)} == {id(a), id(b)}
+        nb.release_staging()
+    assert len(nb._free_stages[0]) == 2 and 1 not in nb._free_stages
+    with pytest.raises(ZeroDivisionError):
+        with nb._host_stage(0):
+            1 / 0
+    assert len(nb._free_stages[0]) == 1
