@@ -4,6 +4,7 @@ definitions and how far a correct result may be off.  Run on the MI355X: -m gpu.
 import copy
 import math
 
+import numpy as np
 import pytest
 import torch
 from torch import nn
@@ -361,3 +362,79 @@ def test_a_cpu_round_within_a_cpu_round():
         want, _, added = no.bounded([[m.w] for m in ms], weights, [ms[0].w], bound)
         no.assert_close(got.w, want[0], 12_000, added[0])
     release_staging()
+
+
+# --------------------------------------------------------------------------- how exact, and the largest forms in full
+@pytest.mark.parametrize("dtype", ["f32", "f64"])
+@pytest.mark.parametrize("n", [1, 2, 9, 16, 130])
+def test_averages_in_64_bits_are_off_by_one_rounding_a_step(n, dtype):
+    """Without a bound the shares are the weights.  In 64 bits the difference, the product with its addition, and the
+    centre's addition round once each: N + 3 times 2^-53 of M = |c| + sum_k |w_k d_k| at most, and then the result by half a
+    step.  The reference is carried in 80 bits, which adds (N + 3) 2^-64 M."""
+    from accdfl_amd.core.norms import wsum_bounded
+
+    (center,), models, weights = _round(n, [20_011], dtype, seed=50, scale=0.5)
+    out, _ = wsum_bounded([m[0] for m in models], weights, center, INF)
+    c = center.cpu().numpy().astype(np.longdouble)
+    want, mag = c.copy(), np.abs(c)
+    for (m,), w in zip(models, weights):
+        d = np.longdouble(w) * (m.cpu().numpy().astype(np.longdouble) - c)
+        want, mag = want + d, mag + np.abs(d)
+    off = np.abs(out.cpu().numpy().astype(np.longdouble) - want)
+    half = torch.finfo(DT[dtype]).eps / 2
+    assert bool((off <= half * np.abs(want) + (n + 3) * (2.0 ** -53 + 2.0 ** -64) * (1 + half) * mag).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "f64"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_clip_beyond_the_infinity_cache_in_full(dtype, in_place):
+    """Over 256 MB a clip streams past the caches: every element, in place and out of place, tensors at odd starts."""
+    from accdfl_amd.core.norms import clip_global_norm
+
+    sizes = [300 * (1 << 20) // DT[dtype].itemsize, 5, 1_000_003]
+    buf = torch.randn(sum(sizes), device="cuda", generator=torch.Generator("cuda").manual_seed(3)).mul_(0.01).to(DT[dtype])
+    ts = list(torch.split(buf, sizes[::-1]))
+    kept = buf.clone()
+    sent = buf if in_place else torch.full_like(buf, 7.0)
+    outs, norm = clip_global_norm(ts, 0.5, outs=list(torch.split(sent, sizes[::-1])))
+    exact = math.sqrt(sum(float(k.double().square().sum()) for k in torch.split(kept, 1 << 24)))
+    no.assert_norm(norm, exact, buf.numel())
+    ratio = 0.5 / (exact + no.CLIP_EPS)
+    # the norm, of up to 1.6e8 terms on either side, is off by 2^-53 of the longest chain of sums: below 2^-30 by far
+    half = torch.finfo(DT[dtype]).eps / 2 + (0.0 if dtype == "f64" else 2.0 ** -24) + 2.0 ** -30
+    least = torch.finfo(DT[dtype]).smallest_normal * torch.finfo(DT[dtype]).eps / 2
+    for s, k in zip(torch.split(sent, 1 << 24), torch.split(kept, 1 << 24)):
+        want = k.double() * ratio
+        assert bool(((s.double() - want).abs() <= half * want.abs() + least).all())
+    if not in_place:
+        assert torch.equal(buf, kept)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "f64"])
+def test_an_average_beyond_the_infinity_cache_in_full(dtype):
+    """Rounds of 8 peers and more over 256 MB run fewer waves at once: every element."""
+    from accdfl_amd.core.norms import wsum_bounded_multi
+
+    n, sizes = 9, [2_700_001 * 4 // DT[dtype].itemsize * 3, 11, 70_001]
+    gen = torch.Generator("cuda").manual_seed(4)
+    make = lambda scale: [torch.randn(s, device="cuda", generator=gen).mul_(scale).to(DT[dtype]) for s in sizes]  # noqa: E731
+    center = make(0.5)
+    models = [[(c + d).to(DT[dtype]) for c, d in zip(center, make(0.01 * (1 + k % 3)))] for k in range(n)]
+    assert sum(sizes) * DT[dtype].itemsize * (n + 1) > 256 << 20
+    weights = [(k + 1) / 45 for k in range(n)]
+    bound = 0.015 * math.sqrt(sum(sizes))
+    outs = [torch.empty_like(c) for c in center]
+    norms = wsum_bounded_multi(models, weights, center, bound, outs)
+    exact = [math.sqrt(sum(float((m.double() - c.double()).square().sum()) for m, c in zip(ms, center))) for ms in models]
+    no.assert_norm(norms, exact, sum(sizes))
+    assert min(exact) < bound < max(exact)
+    info = torch.finfo(DT[dtype])
+    steps = 2.0 ** -30 + (2.0 ** -24 * (n + 3) if DT[dtype].itemsize == 2 else 0.0)  # the norms' own error; 32-bit sums
+    for i, o in enumerate(outs):
+        c = center[i].double()
+        want, mag = c.clone(), c.abs()
+        for ms, a in zip(models, no.shares(exact, weights, bound)):
+            d = a * (ms[i].double() - c)
+            want, mag = want + d, mag + d.abs()
+        half = info.eps / 2 + (0.0 if dtype == "f64" else 2.0 ** -24)
+        assert bool(((o.double() - want).abs() <= half * want.abs() + steps * mag + info.smallest_normal * info.eps / 2).all())
