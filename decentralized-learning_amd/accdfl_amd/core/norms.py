@@ -204,31 +204,45 @@ class _Elements:
         return False
 
 
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    if t.is_contiguous():
+        begin = t.data_ptr()
+        return begin, begin + t.numel() * t.element_size()
+    place = _Elements.of(t)
+    return place.begin, place.end
+
+
 def _refuse_overlaps(lists: List[List[torch.Tensor]], names: Sequence[str], out: int) -> None:
     """The library's rule for any strides: no element of lists[out] is written twice, and none is an element of another
     tensor, but for the tensor in its own place of another list."""
-    places = [[_Elements.of(t) if t.numel() else None for t in ts] for ts in lists]
-    outs = sorted(((p, i) for i, p in enumerate(places[out]) if p), key=lambda o: o[0].begin)
+    own = [_Elements.of(t) if t.numel() else None for t in lists[out]]
+    outs = sorted(((p, i) for i, p in enumerate(own) if p), key=lambda o: o[0].begin)
     for p, i in outs:
         if p.meets_itself():
             raise ValueError("%s tensor %d: an output has elements that share memory" % (names[out], i))
     begins = [p.begin for p, _ in outs]
     reach = list(itertools.accumulate((p.end for p, _ in outs), max))  # of outs[:j + 1]
 
-    def refuse(l, i, place, stop):
+    def refuse(l, i, t, begin, end, stop):
         """Raises if tensor i of list l meets one of outs[:stop]."""
-        j = min(stop, bisect.bisect_left(begins, place.end)) - 1
-        while j >= 0 and reach[j] > place.begin:
-            if outs[j][0].meet(place):
-                raise _lib.DlaggError("%s tensor %d overlaps %s tensor %d" % (names[l], i, names[out], outs[j][1]))
+        place = None
+        j = min(stop, bisect.bisect_left(begins, end)) - 1
+        while j >= 0 and reach[j] > begin:
+            if outs[j][0].end > begin:
+                if place is None:
+                    place = _Elements.of(t)
+                    if l != out and place.same(own[i]):
+                        return
+                if outs[j][0].meet(place):
+                    raise _lib.DlaggError("%s tensor %d overlaps %s tensor %d" % (names[l], i, names[out], outs[j][1]))
             j -= 1
 
     for q, (p, i) in enumerate(outs):
-        refuse(out, i, p, q)
-    for l, ps in enumerate(places):
-        for i, p in enumerate(ps):
-            if l != out and p is not None and not p.same(places[out][i]):
-                refuse(l, i, p, len(outs))
+        refuse(out, i, lists[out][i], p.begin, p.end, q)
+    for l, ts in enumerate(lists):
+        for i, t in enumerate(ts):
+            if l != out and t is not lists[out][i] and own[i]:
+                refuse(l, i, t, *_span(t), len(outs))
 
 
 def _pack_checked(lists: List[List[torch.Tensor]], names: Sequence[str], lead: int, out: int = -1):
