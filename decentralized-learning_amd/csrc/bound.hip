@@ -999,12 +999,14 @@ int norm_clip_impl(int n_tensors, const int* dtypes, const void* const* tensors,
 constexpr int kMostPeers = 2048;
 
 // Peers beside one read of the centre: 8 at most (their loads are all in flight), groups of equal size.  The norms
-// take 1 024 workgroups in all, from 5 groups on as many as run at once (2 per CU): 128 x 21.3 M bf16 852 us, 871
-// with twice as many; with fewer groups the second half evens out the first (16 x ResNet-34 bf16 127, 131 with half).
+// take 1 024 workgroups in all, from 8 groups on as many as run at once (2 per CU), which evens out as well there and keeps
+// fewer rows open (us, 1 024 / 512: 8 groups, 64 x 12 M bf16 257.6 / 250.1 and 64 x 6 M f32 255.1 / 248.8; 16 groups 492.5 /
+// 484.8 and 490.2 / 476.7; but 6 groups 198.5 / 202.9 and 195.2 / 196.7, 5 groups 167.4 / 168.3, 2 groups 71.3 / 73.3, and
+// 40 x ResNet-34 bf16 292 / 298).
 int peer_groups(int n) { return (n + 7) / 8; }
 int64_t peer_blocks(int n) {
   const int groups = peer_groups(n);
-  return std::max(1, (groups > 4 ? 512 : 1024) / groups);
+  return std::max(1, (groups >= 8 ? 512 : 1024) / groups);
 }
 
 int64_t peer_table_words(int64_t n_tensors, int64_t n_peers) {
@@ -1203,9 +1205,10 @@ int round_impl(const char* what, const Round& r, double max_norm, const double* 
   const dim3 grid(static_cast<unsigned>(dla_internal_grid(mean_units, kMeanThreads)));
   // One wave per workgroup and 8 + 1 loads in flight per wave: beyond some 100 KB in flight per CU more waves only
   // keep more DRAM rows open at once.  Rounds of 8 peers and more that read over the Infinity Cache's 256 MB run
-  // 14 waves per CU, by reserving LDS that nothing reads (us, 14 / uncapped: 8 x 25 M f32 157 / 165, 16 x ResNet-34
-  // bf16 128.7 / 130.9, 128 x 2.7 M bf16 127.7 / 130.3); fewer peers lose by it (2 x 25 M f32 74 / 65), smaller
-  // rounds tie (32 x 1.7 M f32 43.3 / 43.0).
+  // 14 waves per CU, by reserving LDS that nothing reads (us, 14 / uncapped: 8 x 25 M f32 157 / 165; reading 800 MB in f32,
+  // 8 peers 137.7 / 153.5, 16 135.1 / 144.8, 32 137.0 / 142.4, 64 135.8 / 135.1; 320 MB, 8 peers 59.1 / 62.1, 16 58.9 / 59.8;
+  // bf16 and f64 alike).  Fewer peers lose by it (4 peers, 800 MB 158.1 / 154.1, 7 peers, 320 MB 63.8 / 59.7), smaller
+  // rounds tie (200 MB, 8 peers 39.6 / 39.2, 32 37.4 / 37.3).
   double bytes = 0;
   for (int t : order) bytes += static_cast<double>(r.numels[t]) * elem_bytes(r.dtypes[t]) * (n + 1);
   const int lds = n >= 8 && bytes > kInfinityCache ? 160 * 1024 / 14 : 0;
