@@ -8,19 +8,22 @@ of a model once before the first element can be written, which is what these ope
     global_norm(tensors)                         one number over a list of tensors
     clip_global_norm(tensors, max_norm)          the list scaled to at most that norm, into new or given tensors
     clip_global_norm_(tensors, max_norm)         the same in place
-    clip_grad_norm_(parameters, max_norm)        the same on parameters' gradients (torch.nn.utils' contract)
+    clip_grad_norm_(parameters, max_norm)        the same on parameters' gradients
     update_norms(models, center)                 how far each model lies from a centre
     wsum_bounded(peers, weights, center, R)      center + sum_k w_k min(1, R / n_k) (peer_k - center), flat peers
     wsum_bounded_multi(...)                      the same over the tensors of whole models
 
 Tensors are float32 / bfloat16 / float16 / float64, mixed freely within a list, on one HIP device, empty ones
 included.  Dense tensors are read where they are whatever the order of their axes and wherever they start; others
-(a slice with gaps, an expanded tensor) are copied first.  Norms and products are carried in 64 bits, averages in 64
-(32 for the 16-bit types, where they hold every term), and rounded once.  Results are on the device and nothing
-synchronises; nothing here is differentiable.  Work is enqueued on ``stream`` or the current stream of the tensors'
-device, workspaces come from torch's caching allocator for each call, and launches take their tables by value (those
-of large rounds from a slot of page-locked memory that the call owns until the GPU has read it; under capture by value
-too): calls on several streams or threads do not meet, and a call captured into a graph replays.
+(a slice with gaps, an expanded tensor) are copied first.  Outputs that overlap each other, themselves or another tensor
+are refused whatever their strides.  Norms and products are carried in 64 bits, averages in 64 (32 for the 16-bit
+types, where they hold every term), and rounded once; a norm beyond float32's range is returned as infinity by
+float32, but is finite for what is scaled by it.  Results are on the device and nothing synchronises; nothing here is
+differentiable.  Work is enqueued on ``stream`` or the current stream of the tensors' device (tensors of another
+stream are the caller's to keep until it has passed), workspaces come from torch's caching allocator for each call, and
+launches take their tables by value (those of large rounds from a slot of page-locked memory that the call owns until
+the GPU has read it; under capture by value too): calls on several streams or threads do not meet, and a call captured
+into a graph replays.
 """
 from __future__ import annotations
 
@@ -365,7 +368,8 @@ def global_norm(tensors: Tensors, norm_type: float = 2.0, error_if_nonfinite: bo
                 stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """The norm of all elements of ``tensors`` (tensors, a module's parameters, or one tensor) as if they were one
     vector: ``norm_type`` 2, 1 or inf.  A scalar on their device, float32 (float64 if any tensor is); 0 for no
-    elements.  NaN anywhere gives NaN; ``error_if_nonfinite`` then raises instead (it waits for the GPU)."""
+    elements.  NaN anywhere gives NaN; ``error_if_nonfinite`` raises where the norm, as it is returned, is NaN or
+    infinite (it waits for the GPU)."""
     code = _norm_code(norm_type)
     tensors = _tensors_of(tensors)
     with _place(_device_of(tensors, stream), stream):
@@ -436,9 +440,10 @@ def clip_global_norm_(tensors: Tensors, max_norm: float, norm_type: float = 2.0,
 
 def clip_grad_norm_(parameters: Tensors, max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
-    """torch.nn.utils.clip_grad_norm_'s contract: the gradients of ``parameters`` (parameters, or a module) clipped
-    in place by their global norm, which is returned.  Parameters without a gradient are skipped; the gradients
-    are on one device, dense and distinct."""
+    """What torch.nn.utils.clip_grad_norm_ does: the gradients of ``parameters`` (parameters, or a module) clipped in
+    place by their global norm, which is returned.  Parameters without a gradient are skipped.  Narrower than torch's:
+    the gradients are on one HIP device, dense and distinct, ``norm_type`` is 1, 2 or inf, and there is no ``foreach``
+    to choose by."""
     grads = [p.grad for p in _tensors_of(parameters)]
     return clip_global_norm_([g for g in grads if g is not None], max_norm, norm_type, error_if_nonfinite)
 
@@ -531,7 +536,7 @@ def wsum_bounded_multi(peer_params: Sequence[Tensors], weights: Sequence[float],
         outs[i] = center[i] + sum_k weights[k] * min(1, max_norm / n_k) * (peer_k[i] - center[i])
 
     in list order, carried in 64 bits (32 for the 16-bit types, where they hold every term) and rounded once.  A peer
-    whose update is not finite (n_k is NaN or infinite) adds nothing.  ``outs[i]`` may be the i-th tensor of the centre
+    whose update is not finite (n_k, in 64 bits, is NaN or infinite) adds nothing.  ``outs[i]`` may be the i-th tensor of the centre
     or of a peer; no other overlap.  ``sq_norms``: float64 squared norms [n] on the device to bound by, when the tensors are one
     bucket of models whose norms are known (update_norms(squared=True), added up).  At most 2 048 peers.  Returns
     the norms [n], float32 (float64 if any tensor is)."""

@@ -228,9 +228,10 @@ int dla_mean(int dtype, const void* const* peers, int n_peers, int64_t n_elems, 
 /* ---- norms over many tensors, and what is bounded by them (additive in ABI v13) ----
  *
  * Tensors are dense and of any of the four dtypes, mixed freely within a call; their pointers need element
- * alignment only.  The sums of norms are carried in 64 bits (F64 elements beyond 1e154 make an infinite norm).
- * Nothing synchronises; the stream's device must be current.  Without a table_host, launches take everything by value except the caller's buffers, so a captured call
- * replays.  The workspaces are the caller's, need no initialisation and hold nothing between calls; two calls in
+ * alignment only.  The sums of norms are carried in 64 bits (F64 elements beyond 1e154 make an infinite norm, those below
+ * 1e-162 count as 0), and what depends on a norm takes it in 64 bits: one beyond F32's range is finite there, although an
+ * F32 result holds it as infinity.  Nothing synchronises; the stream's device must be current.  Without a table_host,
+ * launches take everything by value except the caller's buffers, so a captured call replays.  The workspaces are the caller's, need no initialisation and hold nothing between calls; two calls in
  * flight at once need two.  The counters (NULL: one launch more) let a kernel's last workgroup add up what the others
  * found: DEVICE memory, DLA_COUNTER_BYTES zero bytes, which are zero again when the call's work is done; calls on one
  * stream may share them, calls on two must not. */
@@ -281,7 +282,8 @@ int dla_peer_norms(int n_tensors, const int* dtypes, const void* const* peer_ptr
  *     out = round(c + sum_k a_k (p_k - c)),   a_k = weights[k] * (n_k <= max_norm ? 1 : max_norm / n_k)
  * with n_k as dla_peer_norms gives it, in list order, carried in 64 bits (for BF16 and F16 in 32, rounds with a share or a
  * term beyond their normal range in 64) and rounded once (dla_wsum rounds every step, as the reference does).  A peer
- * whose n_k is not finite adds nothing and is not read.  outs[t] may be tensor t of the centre or of a peer; every other overlap is refused (DLA_E_ALIAS).
+ * whose n_k (in 64 bits) is not finite adds nothing and is not read.  outs[t] may be tensor t of the centre or of a peer;
+ * every other overlap is refused (DLA_E_ALIAS).
  *   sq  DEVICE doubles [n_peers], the squared norms to bound by (a bucket of a model whose norms are known), or
  *       NULL: computed here */
 int dla_wsum_bounded(int n_tensors, const int* dtypes, const void* const* peer_ptrs, const void* const* centers,
