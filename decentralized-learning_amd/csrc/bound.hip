@@ -163,8 +163,8 @@ using Average = std::conditional_t<DT == DLA_BF16 || DT == DLA_F16, Average32, A
 
 // a_k in 32 bits, NaN where 32 bits may not do: a peer's share below their normal range (it would lose bits, or count
 // for nothing), or differences, products or sums beyond it.  |x - c| <= n_k, so n_k <= 2^126 keeps differences in range
-// and |a_k| n_k <= 2^114 the sums over kMostPeers = 2^11 peers.  A NaN makes every sum of the round NaN, and what is NaN is
-// added up again in 64 bits (mean_unit): a round pays for its range only where it needs it.
+// and |a_k| n_k <= 2^114 the sums over kMostPeers = 2^11 peers.  A NaN makes every sum of the round NaN, and what is not
+// finite is added up again in 64 bits (mean_unit): a round pays for its range only where it needs it.
 __device__ inline float share32(double share, double norm) {
   const double a = __builtin_fabs(share);
   const bool fits = a == 0.0 || (a >= 0x1p-126 && a <= 0x1p126 && norm <= 0x1p126 && a * norm <= 0x1p114);
@@ -730,11 +730,11 @@ __device__ inline void mean_unit(const Layout& l, const uint64_t* ptrs, const do
   average<A, DT, 8, TILED>(ptrs, shares, n_peers, center, rc, at, at_c, full, part, acc);
   u32x4 mean = Elem<DT>::narrow(acc);
   if constexpr (std::is_same_v<A, Average32>) {
-    // NaN: a share that 32 bits do not hold, or the data's own, which stays one.  Nothing is written yet, so the output
-    // may be an input here too; one peer at a time, for the registers.
+    // Not finite: a share that 32 bits do not hold, a sum beyond what given norms promised, or the result's own, which
+    // stays so.  Nothing is written yet, so the output may be an input here too; one peer at a time, for the registers.
     bool again = false;
 #pragma unroll
-    for (int e = 0; e < E; ++e) again |= acc[e] != acc[e];
+    for (int e = 0; e < E; ++e) again |= !__builtin_isfinite(acc[e]);
     if (again) {
       double wide[E];
       average<Average64, DT, 1, TILED>(ptrs, shares, n_peers, center, rc, at, at_c, full, part, wide);

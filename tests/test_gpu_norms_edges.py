@@ -131,6 +131,21 @@ def test_a_slab_with_an_outlier(own):
         _assert_average(out[:total], peers, weights, around, bound)
 
 
+@pytest.mark.parametrize("n", [1, 2, 9])
+def test_given_norms_below_the_updates_own(n):
+    """sq_norms are taken as they are: float32's range, which they seem to promise, is passed all the same."""
+    from accdfl_amd.core.norms import wsum_bounded
+
+    c = torch.full((1500,), -3e38, dtype=torch.bfloat16, device="cuda")
+    peers = [torch.full_like(c, 3e38) for _ in range(n)]
+    sq = torch.ones(n, dtype=torch.float64, device="cuda")
+    for weight in (0.25, 1.0):
+        out, norms = wsum_bounded(peers, [weight / n] * n, c, 2.0, sq_norms=sq)
+        want, _, added = no.bounded([[p] for p in peers], [weight / n] * n, [c], 2.0, norms=[1.0] * n)
+        no.assert_close(out, want[0], 1500 + n, added[0])
+        assert bool((norms == 1.0).all())
+
+
 # ------------------------------------------------------------------------------------------ overlapping outputs
 def _overlapping():
     """(name, the tensors to write): each list has an element that is written twice."""
