@@ -553,7 +553,8 @@ def wsum_bounded_multi(peer_params: Sequence[Tensors], weights: Sequence[float],
             return torch.zeros(n, dtype=torch.float32, device=device) if sq_norms is None else sq_norms.sqrt().float()
         tables, back, keep = _pack_round(lists, lambda: ["center", "outs"] + ["peer %d" % k for k in range(n)], 2, out=1)
         if sq_norms is not None and (sq_norms.dtype != torch.float64 or sq_norms.numel() != n
-                                     or sq_norms.device != device or not sq_norms.is_contiguous()):
+                                     or sq_norms.device != device or not sq_norms.is_contiguous()
+                                     or sq_norms.is_neg() or not _held(sq_norms)):
             raise ValueError("sq_norms must be %d contiguous float64 values on %s" % (n, device))
         norms = wsum_bounded_tables(tables, None, [float(w) for w in weights], bound, sq_norms)
         if back:

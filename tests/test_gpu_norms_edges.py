@@ -146,6 +146,17 @@ def test_given_norms_below_the_updates_own(n):
         assert bool((norms == 1.0).all())
 
 
+def test_squared_norms_are_read_from_what_their_storage_holds():
+    from accdfl_amd.core.norms import wsum_bounded
+
+    c, sq = _rand(100), torch.ones(2, dtype=torch.float64, device="cuda")
+    freed = sq.clone()
+    freed.untyped_storage().resize_(0)
+    for bad in (freed, torch._neg_view(sq), sq[:1].expand(2), sq.float()):
+        with pytest.raises(ValueError, match="sq_norms"):
+            wsum_bounded([c, c], [0.5, 0.5], c, 1.0, sq_norms=bad)
+
+
 # ------------------------------------------------------------------------------------------ overlapping outputs
 def _overlapping():
     """(name, the tensors to write): each list has an element that is written twice."""
