@@ -396,8 +396,9 @@ def clip_global_norm(tensors: Tensors, max_norm: float, norm_type: float = 2.0, 
     """(``tensors`` times ``min(1, max_norm / (norm + 1e-6))``, their norm): what a list of tensors becomes under a
     largest global norm, the products rounded once to each tensor's dtype.  ``outs``: tensors of the same sizes
     and dtypes to write (``outs[i]`` may be ``tensors[i]``; no other overlap), else new ones.  A NaN norm makes
-    everything NaN and an infinite one multiplies by 0, as torch.nn.utils.clip_grad_norm_ does;
-    ``error_if_nonfinite`` raises before anything is written instead (it waits for the GPU)."""
+    everything NaN and one that is infinite in 64 bits multiplies by 0, as torch.nn.utils.clip_grad_norm_ does;
+    ``error_if_nonfinite`` raises before anything is written where the norm, as it is returned, is not finite (it waits
+    for the GPU)."""
     code = _norm_code(norm_type)
     bound = _bound(max_norm)
     tensors = _tensors_of(tensors)
@@ -536,10 +537,10 @@ def wsum_bounded_multi(peer_params: Sequence[Tensors], weights: Sequence[float],
         outs[i] = center[i] + sum_k weights[k] * min(1, max_norm / n_k) * (peer_k[i] - center[i])
 
     in list order, carried in 64 bits (32 for the 16-bit types, where they hold every term) and rounded once.  A peer
-    whose update is not finite (n_k, in 64 bits, is NaN or infinite) adds nothing.  ``outs[i]`` may be the i-th tensor of the centre
-    or of a peer; no other overlap.  ``sq_norms``: float64 squared norms [n] on the device to bound by, when the tensors are one
-    bucket of models whose norms are known (update_norms(squared=True), added up).  At most 2 048 peers.  Returns
-    the norms [n], float32 (float64 if any tensor is)."""
+    whose update is not finite (n_k, in 64 bits, is NaN or infinite) adds nothing.  ``outs[i]`` may be the i-th tensor of
+    the centre or of a peer; no other overlap.  ``sq_norms``: float64 squared norms [n] on the device to bound by, when
+    the tensors are one bucket of models whose norms are known (update_norms(squared=True), added up).  At most 2 048
+    peers.  Returns the norms [n], float32 (float64 if any tensor is)."""
     bound = _bound(max_norm)
     outs = _tensors_of(outs)
     lists = [_tensors_of(center_params), outs] + [_tensors_of(p) for p in peer_params]
